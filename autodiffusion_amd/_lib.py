@@ -17,6 +17,7 @@ LIB_PATH = os.environ.get("ADX_LIB_PATH") or os.path.join(_HERE, "libadx.so")   
 ACT_NONE, ACT_RELU, ACT_GELU_ERF, ACT_GELU_TANH, ACT_LEAKY, ACT_SILU, ACT_TANH = range(7)     # ACT_TANH: adx_op_act only
 PREC_F32, PREC_BF16, PREC_BF16X3, PREC_F16X2, PREC_F16 = 0, 1, 2, 3, 4
 PRECISIONS = {"fp32": PREC_F32, "bf16": PREC_BF16, "bf16x3": PREC_BF16X3, "f16x2": PREC_F16X2, "f16": PREC_F16}
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # ADX_DT_*: element types of the operators that take more than fp32
 VARIANT_A, VARIANT_DIT, VARIANT_MMDIT = 0, 1, 2
 FLAG_NORMALIZE, FLAG_RESIDUAL, FLAG_INIT_ZERO, FLAG_NO_GRAPH, FLAG_KEEP_MAPS = 1, 2, 4, 8, 16
 
@@ -35,6 +36,8 @@ EXPORTS = [
     "adx_op_raster_patches", "adx_generate_transition", "adx_op_traj_loss",
     "adx_op_dropout", "adx_op_attention_stats_dropout", "adx_op_attention_bwd_dropout", "adx_op_attention_dropout_mask",
     "adx_op_rmsnorm", "adx_op_rotary", "adx_moe_workspace_bytes", "adx_op_moe_block",
+    "adx_op_rope", "adx_op_linear_residual", "adx_linear_residual_ws_bytes", "adx_op_linear_residual_bwd", "adx_linear_residual_bwd_ws_bytes",
+    "adx_op_moe_few", "adx_moe_few_workspace_bytes",
 ]
 
 
@@ -137,6 +140,13 @@ def load() -> C.CDLL:
         "adx_op_rotary": ([p, p, p, i, i, i, i, i, i, p], i),
         "adx_moe_workspace_bytes": ([i64, i, i, i, i], C.c_size_t),
         "adx_op_moe_block": ([p, p, p, p, p, i64, i, i, i, i, i, p, C.c_size_t, p, p], i),
+        "adx_op_rope": ([p, p, i, p, p, i, p, p, i64, i64, i64, p, f, i, i, i, i, i, i, i, p], i),
+        "adx_op_linear_residual": ([p, i64, p, i64, p, p, i64, p, p, i64, i64, i, i, i, i, p, C.c_size_t, p], i),
+        "adx_linear_residual_ws_bytes": ([i64, i, i, i], C.c_size_t),
+        "adx_op_linear_residual_bwd": ([p, i64, p, i64, p, i64, p, p, p, p, i64, i, i, i, i, p, C.c_size_t, p], i),
+        "adx_linear_residual_bwd_ws_bytes": ([i64, i, i, i, i], C.c_size_t),
+        "adx_op_moe_few": ([p, p, p, p, p, i, i, i, i, i, i, i, p, C.c_size_t, p, p], i),
+        "adx_moe_few_workspace_bytes": ([i, i, i, i, i, i, i], C.c_size_t),
     }
     for name, (args, res) in protos.items():
         fn = getattr(lib, name)
@@ -169,6 +179,34 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def current_stream() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+class on_device:
+    """The tensors' device for the length of a call, its current stream, and the refusal of tensors that are elsewhere: operators run
+    on the stream that is current on the device of their data, whichever device is current for the caller."""
+    __slots__ = ("guard", "stream")
+
+    def __init__(self, what: str, *tensors: Optional[torch.Tensor]):
+        device = None
+        for t in tensors:
+            if t is None:
+                continue
+            if not t.is_cuda:
+                raise AdxError(f"{what}: libadx operates on device memory only; got a CPU tensor")
+            if device is None:
+                device = t.device
+            elif t.device != device:
+                raise AdxError(f"{what}: tensors on {device} and {t.device}")
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self) -> int:
+        if self.guard is not None:
+            self.guard.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 def f32c(t: torch.Tensor) -> torch.Tensor:

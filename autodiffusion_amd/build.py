@@ -16,14 +16,16 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libadx.so")
 OBJ = os.path.join(HERE, "csrc", "build")
-SOURCES = ["kernels.hip", "gemm.hip", "attn_mfma.hip", "modes.hip", "metrics.hip", "extras.hip", "fused_a.hip", "tail_a.hip", "tail_mfma.hip", "engine_base.hip", "engine_a.hip", "engine_dit.hip", "noalloc.hip", "backward.hip", "raster.hip", "moe.hip"]
-HEADERS = ["adx_ops.h", "fastmath.h", "engine.h", os.path.join("..", "..", "include", "adx.h")]
+SOURCES = ["kernels.hip", "gemm.hip", "attn_mfma.hip", "modes.hip", "metrics.hip", "extras.hip", "fused_a.hip", "tail_a.hip", "tail_mfma.hip", "engine_base.hip", "engine_a.hip", "engine_dit.hip", "noalloc.hip", "backward.hip", "raster.hip", "moe.hip", "rope.hip", "product.hip", "moe_few.hip"]
+HEADERS = ["adx_ops.h", "fastmath.h", "typed.h", "engine.h", os.path.join("..", "..", "include", "adx.h")]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wno-unused-function",
          "-Rpass-analysis=kernel-resource-usage"]
+# Sources compiled without packed fp32 arithmetic (v_pk_add / mul / fma_f32).
+NO_PACKED_FP32 = {"rope.hip", "product.hip", "moe_few.hip"}
 # Kernels that must not touch scratch memory: their accumulators or row state live in registers by design, and a loop that stops
 # unrolling (the accumulators are indexed by its counter) silently moves them to scratch -- same results, a quarter slower.
 NO_SCRATCH = re.compile(r"linear_\w*kernel|mlp256_kernel|enc_rows_kernel|attn_g_kernel|tail_mfma_kernel|attn_bf_kernel|attn_mfma\w*kernel|"
-                        r"layernorm_\w*kernel")
+                        r"layernorm_\w*kernel|product_\w*kernel|few_\w*kernel")
 
 
 # known and accepted: the 4-waves-per-SIMD instances of the row kernel (a tuning alternative, not the default) spill a few registers
@@ -67,7 +69,8 @@ def build(force: bool = False, verbose: bool = True, measure: bool = False) -> s
         o = os.path.join(obj_dir, src.replace(".hip", ".o"))
         objs.append(o)
         if force or _stale(o, [s] + hdrs):
-            jobs.append([hipcc, *flags, "-c", s, "-o", o])
+            extra = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] if src in NO_PACKED_FP32 else []
+            jobs.append([hipcc, *flags, *extra, "-c", s, "-o", o])
 
     def run(cmd):
         if verbose:
@@ -78,7 +81,8 @@ def build(force: bool = False, verbose: bool = True, measure: bool = False) -> s
         spilled = [(k, b) for k, b in _scratch_users(r.stderr) if NO_SCRATCH.search(k) and not SCRATCH_OK.search(k)]
         if spilled and not measure:         # the measurement library's ablation instances are exempt
             raise RuntimeError("kernels that must stay in registers use scratch memory:\n" + "\n".join(f"  {k}: {b} bytes per lane" for k, b in spilled))
-        other = "\n".join(l for l in r.stderr.splitlines() if "-Rpass-analysis=kernel-resource-usage" not in l and "remark:" not in l)
+        other = "\n".join(l for l in r.stderr.splitlines() if "-Rpass-analysis=kernel-resource-usage" not in l and "remark:" not in l
+                          and "is not a recognized feature" not in l)     # the host pass does not know the GPU's features
         if verbose and other.strip():
             print(other, file=sys.stderr)
 

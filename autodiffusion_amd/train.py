@@ -819,3 +819,63 @@ def denoise_dit_with_grad(module: torch.nn.Module, x, t, state) -> torch.Tensor:
     meta = (tuple(n for n, _ in named), int(module.config.n_head), len(module.blocks), len(list(module.state_encoder.children())),
             len(list(module.x_encoder.children())), mm, dp)
     return DenoiserDiT.apply(meta, x, t, state, *[p for _, p in named])
+
+
+# ------------------------------------------------------------------------------------------------ decoder-layer operators (fp32 / bf16 / fp16)
+class _Rope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, amplitude, layout):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions if torch.is_tensor(positions) else None, inv_freq)
+        ctx.first, ctx.amplitude, ctx.layout = (None if torch.is_tensor(positions) else positions), amplitude, layout
+        qo, ko = ops.rope(q, k, positions, inv_freq, amplitude, layout)
+        return qo if k is None else (qo, ko)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk=None):
+        positions, inv_freq = ctx.saved_tensors
+        at = ctx.first if positions is None else positions
+        if dq is None and dk is None:
+            return None, None, None, None, None, None
+        if dq is None:                                   # only the keys' outputs were used
+            dk, _ = ops.rope(dk, None, at, inv_freq, ctx.amplitude, ctx.layout, inverse=True)
+        else:
+            dq, dk = ops.rope(dq, dk, at, inv_freq, ctx.amplitude, ctx.layout, inverse=True)
+        return dq, dk, None, None, None, None
+
+
+def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions, inv_freq: torch.Tensor, amplitude: float = 1.0, layout: str = "half"):
+    """``ops.rope`` with gradients: (q', k') -- (q', None) without k.  The gradient is the transposed rotation of the outputs' gradients."""
+    if k is None:
+        return _Rope.apply(q, None, positions, inv_freq, amplitude, layout), None
+    return _Rope.apply(q, k, positions, inv_freq, amplitude, layout)
+
+
+class _LinearResidual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, residual, act_code):
+        need = any(ctx.needs_input_grad[:3])
+        pre = None
+        if need and act_code != _lib.ACT_NONE:
+            y, pre = ops.linear_residual(x, w, bias, residual, act_code, keep_pre=True)
+        else:
+            y = ops.linear_residual(x, w, bias, residual, act_code)
+        ctx.act_code = act_code
+        ctx.save_for_backward(x if need else None, w if need else None, pre)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, pre = ctx.saved_tensors
+        dx = dw = db = None
+        if x is not None:
+            dx, dw, db = ops.linear_residual_bwd(dy, x, w, pre, ctx.act_code, *ctx.needs_input_grad[:3])
+        return dx, dw, db, dy if ctx.needs_input_grad[3] else None, None
+
+
+def linear_residual(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+                    act: int = _lib.ACT_NONE) -> torch.Tensor:
+    """``ops.linear_residual`` with gradients for x, w, bias and residual.  The value before the activation is kept in the tensors' type."""
+    return _LinearResidual.apply(x, w, bias, residual, act)

@@ -47,6 +47,8 @@ enum { ADX_PREC_F32 = 0, ADX_PREC_BF16 = 1, ADX_PREC_BF16X3 = 2,
         * tensors those kernels exchange through memory (cached attention outputs, gates, LayerNorm rows) are stored as fp16; the
         * per-chunk caches, the tail and the scheduler run as under ADX_PREC_BF16X3. */
        ADX_PREC_F16 = 4 };
+/* Element types of the operators that take more than fp32 tensors. */
+enum { ADX_DT_F32 = 0, ADX_DT_BF16 = 1, ADX_DT_F16 = 2 };
 enum { ADX_VARIANT_A = 0, ADX_VARIANT_DIT = 1, ADX_VARIANT_MMDIT = 2 };
 
 /* sampling flags */
@@ -287,6 +289,48 @@ int adx_op_rotary(float* x, const float* cos_table, const float* sin_table, int 
 size_t adx_moe_workspace_bytes(int64_t T, int d, int inter, int E, int top_k);
 int adx_op_moe_block(const float* x, const float* res, const float* router_w, const void* w13, const void* w2, int64_t T, int d, int inter,
                      int E, int top_k, int precision, void* workspace, size_t workspace_bytes, float* y, void* stream);
+
+/* --------------------------------------------------------------------------------------------
+ * Operators of a decoder layer on fp32, bf16 or fp16 tensors (`dtype`: ADX_DT_*).  Sums are fp32, results are rounded once.  The
+ * reference has no counterpart for the types, layouts and gradients (its decoder is third-party `transformers`, see above).
+ * ------------------------------------------------------------------------------------------ */
+/* Rotary positions of queries q[B][S][heads_q][dh] and, unless k is NULL (then heads_k = 0), keys k[B][S][heads_k][dh] in one launch.
+ * The first rotary_dim (even, <= dh, <= 4096) values of every head are turned in pairs (j, j + rotary_dim / 2), or (2 j, 2 j + 1) with
+ * interleaved != 0, by the angle p * inv_freq[j] of the token's position p, and scaled by `amplitude`:
+ *     (a, b) -> amplitude (a cos - b sin, b cos + a sin);  inverse != 0: the transpose (angle negated), which is the gradient.
+ * The other values are copied.  inv_freq[rotary_dim / 2]: fp64, radians a position (any scaling for long contexts is in it); angles are
+ * computed in 64 bits.  Position of token (b, s): positions[b * pos_stride_b + s * pos_stride_s], or pos0 + s if positions is NULL.
+ * strides_host[12] (host memory): element strides of batch item, token and head of q, q_out, k, k_out; values of a head are adjacent.
+ * An output is its input (same pointer and strides: in place) or does not overlap any input. */
+int adx_op_rope(const void* q, void* q_out, int heads_q, const void* k, void* k_out, int heads_k, const int64_t* strides_host,
+                const int64_t* positions, int64_t pos_stride_b, int64_t pos_stride_s, int64_t pos0, const double* inv_freq, float amplitude,
+                int B, int S, int dh, int rotary_dim, int interleaved, int inverse, int dtype, void* stream);
+/* y[M][N] = act(x[M][K] w[N][K]^T + bias[N]) + res[M][N]; bias, res nullable; all tensors of one element type; row strides (elements)
+ * ldx, ldw, ldr, ldy >= N, adjacent values in a row (ldr = 0: one row for all).  pre (nullable, [M][N] contiguous) receives the value
+ * before the activation, which the gradient needs for act != ADX_ACT_NONE.  act: ADX_ACT_NONE .. ADX_ACT_TANH.  y and pre overlap no input,
+ * except that y may be res itself (same pointer and stride).  M = 0 does nothing.
+ * workspace: adx_linear_residual_ws_bytes(M, N, K, dtype) bytes, 16-byte aligned (0: may be NULL), the call's own until it has run. */
+size_t adx_linear_residual_ws_bytes(int64_t M, int N, int K, int dtype);
+int adx_op_linear_residual(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldr, void* pre,
+                           void* y, int64_t ldy, int64_t M, int N, int K, int act, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+/* Its gradients, any of them NULL where not wanted: with dz = dy act'(pre), dx[M][K] = dz w, dw[N][K] = dz^T x, db[N] = column sums of
+ * dz (the residual's gradient is dy itself).  pre may be NULL for ADX_ACT_NONE.  dz is rounded to the element type as the operand of the two
+ * products; db sums the unrounded values.  Sums over rows are joined in a fixed order (no atomics): bit-identical re-runs. */
+size_t adx_linear_residual_bwd_ws_bytes(int64_t M, int N, int K, int act, int dtype);
+int adx_op_linear_residual_bwd(const void* dy, int64_t ldd, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* pre, void* dx,
+                               void* dw, void* db, int64_t M, int N, int K, int act, int dtype, void* workspace, size_t workspace_bytes,
+                               void* stream);
+/* adx_op_moe_block for a few tokens (1 <= T <= 64; d, inter multiples of 32): the same expert layer in two kernels (three where the
+ * routing is large) that read the chosen experts' weights once.  x, res (nullable), y: [T][d] of act_type; router_w [E][d] fp32; w13, w2 as
+ * for adx_op_moe_block under `precision`: fp32 tokens with ADX_PREC_F32, BF16, BF16X3 or F16 (fp16 bits) weights, bf16 tokens with
+ * ADX_PREC_BF16, fp16 tokens with ADX_PREC_F16.  Tokens and hidden values are not rounded below their fp32 accuracy (16-bit act_type:
+ * 2^-16).  The routing is that of adx_op_moe_block and is left at the head of the workspace the same way (T * top_k int32, then
+ * from the next multiple of 256 bytes T * top_k floats); a token whose router probabilities are NaN goes to the first experts.
+ * workspace: adx_moe_few_workspace_bytes bytes, 16-byte aligned, contents arbitrary, the call's own until it has run.  No host
+ * synchronisation; the order of every sum is fixed. */
+size_t adx_moe_few_workspace_bytes(int T, int d, int inter, int E, int top_k, int act_type, int precision);
+int adx_op_moe_few(const void* x, const void* res, const float* router_w, const void* w13, const void* w2, int T, int d, int inter, int E,
+                   int top_k, int act_type, int precision, void* workspace, size_t workspace_bytes, void* y, void* stream);
 
 /* --------------------------------------------------------------------------------------------
  * Operators of the training paths (fp32): the refiner, the flattened wrapper and the decoder twin.  The reference differentiates
