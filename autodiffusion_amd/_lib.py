@@ -6,6 +6,7 @@ exception is raised.  Nothing in this package computes the hot path on the CPU.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from typing import Optional
 
@@ -181,32 +182,45 @@ def current_stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
-class on_device:
-    """The tensors' device for the length of a call, its current stream, and the refusal of tensors that are elsewhere: operators run
-    on the stream that is current on the device of their data, whichever device is current for the caller."""
-    __slots__ = ("guard", "stream")
+def device_of(what: str, *tensors: Optional[torch.Tensor]) -> int:
+    """Index of the one device that holds all tensors (None skipped); refuses host tensors and tensors on several devices."""
+    device = -2
+    for t in tensors:
+        if t is not None:
+            at = t.get_device()                          # -1: host memory
+            if at != device:
+                if at < 0:
+                    raise AdxError(f"{what}: libadx operates on device memory only; got a CPU tensor")
+                if device >= 0:
+                    raise AdxError(f"{what}: tensors on cuda:{device} and cuda:{at}")
+                device = at
+    return device
 
-    def __init__(self, what: str, *tensors: Optional[torch.Tensor]):
-        device = None
-        for t in tensors:
-            if t is None:
-                continue
-            if not t.is_cuda:
-                raise AdxError(f"{what}: libadx operates on device memory only; got a CPU tensor")
-            if device is None:
-                device = t.device
-            elif t.device != device:
-                raise AdxError(f"{what}: tensors on {device} and {t.device}")
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
-    def __enter__(self) -> int:
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
+def on_data_device(fn):
+    """For operators whose first steps are ``device_of`` and ``stream_on``: when another device than the data's is current, the call is made
+    again with theirs current, so that it runs on the stream that is current there."""
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        try:
+            return fn(*args, **kwargs)
+        except _OtherDevice as other:
+            index = other.index
+        with torch.cuda.device(index):
+            return fn(*args, **kwargs)
+    return call
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+
+class _OtherDevice(Exception):
+    def __init__(self, index: int):
+        self.index = index
+
+
+def stream_on(index: int) -> int:
+    """The current stream of device ``index``, which has to be the current device (else ``on_data_device`` makes it that)."""
+    if index != torch.cuda.current_device():
+        raise _OtherDevice(index)
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def f32c(t: torch.Tensor) -> torch.Tensor:

@@ -8,7 +8,7 @@
 //   2. down  workgroup = (16 output columns, a share of the (expert, K piece) units): weighted products added per token; with more than
 //            one share the last workgroup of a column group to finish adds the shares in order -- the order of the sums never depends
 //            on timing.
-// The routing of all tokens is computed by every workgroup of `up` itself while that costs less than a launch (ROUTE_INSIDE),
+// The routing of all tokens is computed by every workgroup of `up` itself while that costs less than a launch (ROUTE_INSIDE below),
 // otherwise by a kernel of its own in front.
 //
 // Precision.  Sums are fp32.  The hidden values stay at fp32 accuracy: they are kept as two (16-bit outputs, 2^-17) or three (fp32
@@ -17,6 +17,7 @@
 // the fp16 range stay finite.
 #include "adx_ops.h"
 #include "engine.h"
+#include "fastmath.h"
 #include "typed.h"
 
 #include <type_traits>
@@ -26,7 +27,6 @@ namespace {
 
 constexpr int FEW_MAX_T = 64, FEW_MAX_K = 8, FEW_MAX_E = 64;
 constexpr int WAVES = 8;                                  // of a workgroup of either product
-constexpr int64_t ROUTE_INSIDE = 1 << 18;                 // T * E * d up to which `up` routes by itself
 enum : int { P_F32 = 0, P_BF16 = 1, P_BF16X3 = 2, P_F16 = 4 };         // the ADX_PREC_* codes
 
 struct FewArgs {
@@ -34,21 +34,37 @@ struct FewArgs {
     const void* w13; const void* w2;
     int T, d, inter, E, top_k;
     int* idx; float* wts;                                 // [T][top_k]
+    int* table; int active;                               // `up` -> `down`: [active] rows of {expert or -1, count, entries (token * top_k + slot)[T]}
     void* h; int64_t h_plane;                             // hidden rows [part][T top_k][inter]; elements of one part
     float* part; int* arrived;                            // shares > 1: [shares][T][d], [d / 16]
     int shares, k_splits;
     void* y;
 };
 
+// Reductions over a wave by data-parallel moves: pairs and quads, the mirrored halves of 8 and 16 lanes, then the row and half swaps --
+// vector instructions of a few cycles each, where a shuffle is a round trip through the LDS crossbar.
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
+}
+constexpr int QUAD_SWAP1 = 0xB1, QUAD_SWAP2 = 0x4E, HALF_MIRROR = 0x141, MIRROR = 0x140;
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+    v += dpp<QUAD_SWAP1>(v);
+    v += dpp<QUAD_SWAP2>(v);
+    v += dpp<HALF_MIRROR>(v);
+    v += dpp<MIRROR>(v);
+    return xor32_add(xor16_add(v));
+}
+__device__ __forceinline__ float xor16_max(float x) {
+    const unsigned u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+    v = fmaxf(v, dpp<QUAD_SWAP1>(v));
+    v = fmaxf(v, dpp<QUAD_SWAP2>(v));
+    v = fmaxf(v, dpp<HALF_MIRROR>(v));
+    v = fmaxf(v, dpp<MIRROR>(v));
+    return xor32_max(xor16_max(v));
 }
 
 // ------------------------------------------------------------------------------------------------------------- operand fragments
@@ -134,26 +150,42 @@ __device__ __forceinline__ f32x4_t mfma_parts(const uint4 (&w)[PW], const uint4 
 }
 
 // ------------------------------------------------------------------------------------------------------------- routing
-// logits of tokens t0 .. t0 + n - 1 into `logit` [n][E], one (token, expert) pair a wave at a time, then the choice, one token a wave.
+// The routing of tokens t0 .. t0 + n - 1 by a whole workgroup: every wave takes its part of the summed axis of one token and eight
+// experts, so that the loads of a logit are one round trip; then the choice, one token a wave.  `part`: n ceil(E / 8) * 64 floats of LDS.
+constexpr int ROUTE_GROUPS = 8;                           // tokens times groups of eight experts a call may hold in LDS
 template <typename A>
-__device__ __forceinline__ void route(const FewArgs& a, int t0, int n, float* logit, int* idx, float* wts) {
+__device__ __forceinline__ void route(const FewArgs& a, int t0, int n, float* part, int* idx, float* wts) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int p = wave; p < n * a.E; p += WAVES) {
-        const int t = p / a.E, e = p - t * a.E;
+    const int groups = (a.E + 7) / 8;
+    for (int p = 0; p < n * groups; ++p) {
+        const int t = p / groups, e0 = (p - t * groups) * 8;
         const A* x = static_cast<const A*>(a.x) + (int64_t)(t0 + t) * a.d;
-        const float* w = a.router + (int64_t)e * a.d;
-        float s = 0.f;
-        for (int i = lane * 4; i < a.d; i += 256) {                    // d is a multiple of 32
+        float s[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s[q] = 0.f;
+        for (int i = threadIdx.x * 4; i < a.d; i += 256 * WAVES) {      // d is a multiple of 32
             const Pack<A, 4> xv = *reinterpret_cast<const Pack<A, 4>*>(x + i);
-            const float4 wv = *reinterpret_cast<const float4*>(w + i);
-            s += (float)xv.v[0] * wv.x + (float)xv.v[1] * wv.y + (float)xv.v[2] * wv.z + (float)xv.v[3] * wv.w;
+            float4 wv[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) wv[q] = *reinterpret_cast<const float4*>(a.router + (int64_t)min(e0 + q, a.E - 1) * a.d + i);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) s[q] += (float)xv.v[0] * wv[q].x + (float)xv.v[1] * wv[q].y + (float)xv.v[2] * wv[q].z + (float)xv.v[3] * wv[q].w;
         }
-        s = wave_sum(s);
-        if (lane == 0) logit[p] = s;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            s[q] = wave_sum(s[q]);
+            if (lane == 0) part[(p * WAVES + wave) * 8 + q] = s[q];
+        }
     }
     __syncthreads();
     for (int t = wave; t < n; t += WAVES) {
-        const float mine = lane < a.E ? logit[t * a.E + lane] : -INFINITY;
+        float mine = -INFINITY;
+        if (lane < a.E) {
+            const float* l = part + (t * groups + (lane >> 3)) * WAVES * 8 + (lane & 7);
+            mine = 0.f;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) mine += l[w * 8];
+        }
         const float mx = wave_max(mine);
         const float ex = lane < a.E ? expf(mine - mx) : 0.f;
         const float p = ex / wave_sum(ex);
@@ -178,9 +210,9 @@ __device__ __forceinline__ void route(const FewArgs& a, int t0, int n, float* lo
 
 template <typename A>
 __global__ __launch_bounds__(64 * WAVES) void few_route_kernel(const FewArgs a) {
-    __shared__ float logit[FEW_MAX_E];
+    __shared__ float part[ROUTE_GROUPS * WAVES * 8];
     const int t = blockIdx.x;
-    route<A>(a, t, 1, logit, a.idx + t * a.top_k, a.wts + t * a.top_k);
+    route<A>(a, t, 1, part, a.idx + t * a.top_k, a.wts + t * a.top_k);
 }
 
 // The `rank`-th expert (by index) that any token chose, -1 if there are fewer; its entries (token * top_k + slot) in token order
@@ -216,8 +248,9 @@ __device__ __forceinline__ void entries_of(const int* idx, int n, int e, Chosen&
 }
 
 // ------------------------------------------------------------------------------------------------------------- gate and up
+// Tokens of an expert are taken 16 MT at a time; a second pass finds the weights in the L2.
 template <typename A, int P, int MT, bool INSIDE>
-__global__ __launch_bounds__(64 * WAVES) void few_up_kernel(const FewArgs a) {
+__global__ __launch_bounds__(64 * WAVES, (P == P_F32 || sizeof(A) == 2) ? 4 : 2) void few_up_kernel(const FewArgs a) {
     typedef Weight<P> W;
     constexpr int CE = W::CE, PIECE = 8 * CE;                            // 128 bytes of a 16-bit or fp32 row
     constexpr bool RAW_X = P == P_F32 || sizeof(A) == 2;                 // token values go into the matrix instruction as they are
@@ -229,7 +262,8 @@ __global__ __launch_bounds__(64 * WAVES) void few_up_kernel(const FewArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g = lane >> 4;
     const int n = a.T * a.top_k;
     if constexpr (INSIDE) {
-        route<A>(a, 0, a.T, &sums[0][0][0][0], idx_s, wts_s);            // T * E <= 4096 logits fit the sums' space
+        static_assert(ROUTE_GROUPS * WAVES * 8 <= WAVES * 2 * 64 * 4, "the routing's sums fit");
+        route<A>(a, 0, a.T, &sums[0][0][0][0], idx_s, wts_s);
         if (blockIdx.x == 0 && blockIdx.y == 0)
             for (int i = tid; i < n; i += 64 * WAVES) { a.idx[i] = idx_s[i]; a.wts[i] = wts_s[i]; }
     } else {
@@ -239,88 +273,99 @@ __global__ __launch_bounds__(64 * WAVES) void few_up_kernel(const FewArgs a) {
         for (int i = tid; i < a.d / 16; i += 64 * WAVES) a.arrived[i] = 0;
     __syncthreads();
     const int e = chosen_expert(idx_s, n, blockIdx.y, ch.used);
-    if (e < 0) return;
+    int* row_of_table = a.table + (int64_t)blockIdx.y * (a.T + 2);
+    if (e < 0) {
+        if (blockIdx.x == 0 && tid == 0) row_of_table[0] = -1;
+        return;
+    }
     entries_of(idx_s, n, e, ch);
     const int count = ch.count, col0 = blockIdx.x * 16;
+    if (blockIdx.x == 0) {
+        if (tid < count) row_of_table[2 + tid] = ch.entry[tid];
+        if (tid == 0) { row_of_table[0] = e; row_of_table[1] = count; }
+    }
     const int64_t low = (int64_t)a.E * 2 * a.inter * a.d;
     const int64_t gate = ((int64_t)e * 2 * a.inter + col0 + r16) * a.d + g * CE, up = gate + (int64_t)a.inter * a.d;
-    const A* x[MT];
-    bool live[MT];
+    for (int m0 = 0; m0 < count; m0 += 16 * MT) {
+        const A* x[MT];
+        bool live[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        live[t] = t * 16 + r16 < count;
-        x[t] = static_cast<const A*>(a.x) + (int64_t)(live[t] ? ch.entry[t * 16 + r16] / a.top_k : 0) * a.d + g * CE;
-    }
-    f32x4_t acc[2][MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) acc[0][t] = acc[1][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    constexpr int U = 2;                                                  // half pieces (64 bytes a row) in flight: 2 U
-    const int K = a.d - g * CE;
-    for (int k = wave * PIECE; k < a.d; k += U * WAVES * PIECE) {
-        W w[2 * U][2];
-        uint4 xv[2 * U][MT][RAW_X ? 1 : 2];
-#pragma unroll
-        for (int q = 0; q < 2 * U; ++q) {
-            const int kq = k + (q >> 1) * WAVES * PIECE + (q & 1) * 4 * CE;
-            const bool ok = kq < K;
-            if (ok) { w[q][0].load(a.w13, gate + kq, low); w[q][1].load(a.w13, up + kq, low); }
-            else { w[q][0].clear(); w[q][1].clear(); }
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-#pragma unroll
-                for (int z = 0; z < (RAW_X ? 1 : 2); ++z)
-                    xv[q][t][z] = ok && live[t] ? *reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned char*>(x[t] + kq) + 16 * z) : make_uint4(0u, 0u, 0u, 0u);
-            }
+        for (int t = 0; t < MT; ++t) {
+            live[t] = m0 + t * 16 + r16 < count;
+            x[t] = static_cast<const A*>(a.x) + (int64_t)(live[t] ? ch.entry[m0 + t * 16 + r16] / a.top_k : 0) * a.d + g * CE;
         }
+        f32x4_t acc[2][MT];
 #pragma unroll
-        for (int q = 0; q < 2 * U; ++q) {
+        for (int t = 0; t < MT; ++t) acc[0][t] = acc[1][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        constexpr int U = 2;                                              // pieces in flight a wave
+        const int K = a.d - g * CE;
+        for (int k = wave * PIECE; k < a.d; k += U * WAVES * PIECE) {
+            W w[2 * U][2];
+            uint4 xv[2 * U][MT][RAW_X ? 1 : 2];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                if constexpr (P == P_F32) {
-                    acc[0][t] = mfma_f(w[q][0].raw[0], xv[q][t][0], acc[0][t]);
-                    acc[1][t] = mfma_f(w[q][1].raw[0], xv[q][t][0], acc[1][t]);
-                } else if constexpr (RAW_X && P == P_BF16) {
-                    acc[0][t] = mfma_bf(w[q][0].raw[0], xv[q][t][0], acc[0][t]);
-                    acc[1][t] = mfma_bf(w[q][1].raw[0], xv[q][t][0], acc[1][t]);
-                } else if constexpr (RAW_X) {
-                    acc[0][t] = mfma_h(w[q][0].raw[0], xv[q][t][0], acc[0][t]);
-                    acc[1][t] = mfma_h(w[q][1].raw[0], xv[q][t][0], acc[1][t]);
-                } else {
-                    const float v[8] = {__uint_as_float(xv[q][t][0].x), __uint_as_float(xv[q][t][0].y), __uint_as_float(xv[q][t][0].z), __uint_as_float(xv[q][t][0].w),
-                                        __uint_as_float(xv[q][t][1].x), __uint_as_float(xv[q][t][1].y), __uint_as_float(xv[q][t][1].z), __uint_as_float(xv[q][t][1].w)};
-                    uint4 px[PX], pw[W::PARTS];
-                    split8<PX>(v, px);
+            for (int q = 0; q < 2 * U; ++q) {
+                const int kq = k + (q >> 1) * WAVES * PIECE + (q & 1) * 4 * CE;
+                const bool ok = kq < K;
+                if (ok) { w[q][0].load(a.w13, gate + kq, low); w[q][1].load(a.w13, up + kq, low); }
+                else { w[q][0].clear(); w[q][1].clear(); }
 #pragma unroll
-                    for (int z = 0; z < 2; ++z) {
-                        w[q][z].parts(pw);
-                        acc[z][t] = mfma_parts<W::PARTS, PX, 3>(pw, px, acc[z][t]);
+                for (int t = 0; t < MT; ++t) {
+#pragma unroll
+                    for (int z = 0; z < (RAW_X ? 1 : 2); ++z)
+                        xv[q][t][z] = ok && live[t] ? *reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned char*>(x[t] + kq) + 16 * z) : make_uint4(0u, 0u, 0u, 0u);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 2 * U; ++q) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    if constexpr (P == P_F32) {
+                        acc[0][t] = mfma_f(w[q][0].raw[0], xv[q][t][0], acc[0][t]);
+                        acc[1][t] = mfma_f(w[q][1].raw[0], xv[q][t][0], acc[1][t]);
+                    } else if constexpr (RAW_X && P == P_BF16) {
+                        acc[0][t] = mfma_bf(w[q][0].raw[0], xv[q][t][0], acc[0][t]);
+                        acc[1][t] = mfma_bf(w[q][1].raw[0], xv[q][t][0], acc[1][t]);
+                    } else if constexpr (RAW_X) {
+                        acc[0][t] = mfma_h(w[q][0].raw[0], xv[q][t][0], acc[0][t]);
+                        acc[1][t] = mfma_h(w[q][1].raw[0], xv[q][t][0], acc[1][t]);
+                    } else {
+                        const float v[8] = {__uint_as_float(xv[q][t][0].x), __uint_as_float(xv[q][t][0].y), __uint_as_float(xv[q][t][0].z), __uint_as_float(xv[q][t][0].w),
+                                            __uint_as_float(xv[q][t][1].x), __uint_as_float(xv[q][t][1].y), __uint_as_float(xv[q][t][1].z), __uint_as_float(xv[q][t][1].w)};
+                        uint4 px[PX], pw[W::PARTS];
+                        split8<PX>(v, px);
+#pragma unroll
+                        for (int z = 0; z < 2; ++z) {
+                            w[q][z].parts(pw);
+                            acc[z][t] = mfma_parts<W::PARTS, PX, 3>(pw, px, acc[z][t]);
+                        }
                     }
                 }
             }
         }
-    }
-    __syncthreads();                                                      // the routing's use of `sums` is over
+        __syncthreads();                                                  // what `sums` held before has been read
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        *reinterpret_cast<f32x4_t*>(sums[wave][2 * t][lane]) = acc[0][t];
-        *reinterpret_cast<f32x4_t*>(sums[wave][2 * t + 1][lane]) = acc[1][t];
-    }
-    __syncthreads();
-    // result layout of the 16x16 product: column (token) = lane & 15, row (hidden column) = 4 (lane >> 4) + reg
-    for (int i = tid; i < count * 16; i += 64 * WAVES) {
-        const int m = i >> 4, c = i & 15, t = m >> 4, l = (c >> 2) * 16 + (m & 15);
-        float vg = 0.f, vu = 0.f;
+        for (int t = 0; t < MT; ++t) {
+            *reinterpret_cast<f32x4_t*>(sums[wave][2 * t][lane]) = acc[0][t];
+            *reinterpret_cast<f32x4_t*>(sums[wave][2 * t + 1][lane]) = acc[1][t];
+        }
+        __syncthreads();
+        // result layout of the 16x16 product: column (token) = lane & 15, row (hidden column) = 4 (lane >> 4) + reg
+        const int rows = min(count - m0, 16 * MT);
+        for (int i = tid; i < rows * 16; i += 64 * WAVES) {
+            const int m = i >> 4, c = i & 15, t = m >> 4, l = (c >> 2) * 16 + (m & 15);
+            float vg = 0.f, vu = 0.f;
 #pragma unroll
-        for (int s = 0; s < WAVES; ++s) { vg += sums[s][2 * t][l][c & 3]; vu += sums[s][2 * t + 1][l][c & 3]; }
-        float v = vg / (1.f + expf(-vg)) * vu;
-        const int64_t at = (int64_t)ch.entry[m] * a.inter + col0 + c;
-        if constexpr (P == P_F32) static_cast<float*>(a.h)[at] = v;
-        else {
+            for (int s = 0; s < WAVES; ++s) { vg += sums[s][2 * t][l][c & 3]; vu += sums[s][2 * t + 1][l][c & 3]; }
+            float v = vg / (1.f + expf(-vg)) * vu;
+            const int64_t at = (int64_t)ch.entry[m0 + m] * a.inter + col0 + c;
+            if constexpr (P == P_F32) static_cast<float*>(a.h)[at] = v;
+            else {
 #pragma unroll
-            for (int p = 0; p < PH; ++p) {
-                const __bf16 b = (__bf16)v;
-                static_cast<__bf16*>(a.h)[p * a.h_plane + at] = b;
-                v = __builtin_isfinite((float)b) ? v - (float)b : 0.f;
+                for (int p = 0; p < PH; ++p) {
+                    const __bf16 b = (__bf16)v;
+                    static_cast<__bf16*>(a.h)[p * a.h_plane + at] = b;
+                    v = __builtin_isfinite((float)b) ? v - (float)b : 0.f;
+                }
             }
         }
     }
@@ -328,76 +373,78 @@ __global__ __launch_bounds__(64 * WAVES) void few_up_kernel(const FewArgs a) {
 
 // ------------------------------------------------------------------------------------------------------------- down
 template <typename A, int P, int MT>
-__global__ __launch_bounds__(64 * WAVES) void few_down_kernel(const FewArgs a) {
+__global__ __launch_bounds__(64 * WAVES, (P == P_F32 || sizeof(A) == 2) ? 4 : 2) void few_down_kernel(const FewArgs a) {
     typedef Weight<P> W;
     constexpr int CE = W::CE, PIECE = 8 * CE, PH = P == P_F32 ? 1 : sizeof(A) == 4 ? 3 : 2;
-    __shared__ float ysum[WAVES][MT * 16][16 + 1];
-    __shared__ int idx_s[FEW_MAX_T * FEW_MAX_K];
-    __shared__ float wts_s[FEW_MAX_T * FEW_MAX_K];
-    __shared__ Chosen ch;
+    constexpr int ROWS = MT == 1 ? 16 : FEW_MAX_T;                        // tokens the launch may have
+    __shared__ float ysum[WAVES][ROWS][16 + 1];
     __shared__ int last;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g = lane >> 4;
-    const int n = a.T * a.top_k, col0 = blockIdx.x * 16;
-    for (int i = tid; i < n; i += 64 * WAVES) { idx_s[i] = a.idx[i]; wts_s[i] = a.wts[i]; }
-    for (int i = lane; i < MT * 16 * 17; i += 64) (&ysum[wave][0][0])[i] = 0.f;
+    const int col0 = blockIdx.x * 16;
+    for (int i = lane; i < ROWS * 17; i += 64) (&ysum[wave][0][0])[i] = 0.f;
     __syncthreads();
     const int64_t low = (int64_t)a.E * a.inter * a.d;
     // unit u = (chosen expert u / k_splits, part u % k_splits of the hidden axis); this workgroup takes every shares-th
     const int piece_len = (a.inter + a.k_splits * PIECE - 1) / (a.k_splits * PIECE) * PIECE;
-    for (int u = blockIdx.y;; u += a.shares) {
-        const int e = chosen_expert(idx_s, n, u / a.k_splits, ch.used);
+    for (int u = blockIdx.y; u < a.active * a.k_splits; u += a.shares) {
+        const int* row_of_table = a.table + (int64_t)(u / a.k_splits) * (a.T + 2);
+        const int e = row_of_table[0];
         if (e < 0) break;
-        entries_of(idx_s, n, e, ch);
-        const int count = ch.count, k_lo = (u % a.k_splits) * piece_len, k_hi = min(k_lo + piece_len, a.inter);
+        const int count = row_of_table[1], k_lo = (u % a.k_splits) * piece_len, k_hi = min(k_lo + piece_len, a.inter);
         const int64_t row = ((int64_t)e * a.d + col0 + r16) * a.inter + g * CE;
-        int64_t h[MT];
-        bool live[MT];
+        for (int m0 = 0; m0 < count; m0 += 16 * MT) {
+            int64_t h[MT];
+            int entry[MT];
+            float wt[MT];
+            bool live[MT];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            live[t] = t * 16 + r16 < count;
-            h[t] = (int64_t)(live[t] ? ch.entry[t * 16 + r16] : 0) * a.inter + g * CE;
-        }
-        f32x4_t acc[MT];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        constexpr int U = MT == 1 ? 4 : MT * PH >= 8 ? 1 : 2;         // registers
-        const int K = k_hi - g * CE;
-        for (int k = k_lo + wave * PIECE; k < k_hi; k += U * WAVES * PIECE) {
-            W w[2 * U];
-            uint4 hv[2 * U][MT][PH];
-#pragma unroll
-            for (int q = 0; q < 2 * U; ++q) {
-                const int kq = k + (q >> 1) * WAVES * PIECE + (q & 1) * 4 * CE;
-                const bool ok = kq < K;
-                if (ok) w[q].load(a.w2, row + kq, low);
-                else w[q].clear();
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
-#pragma unroll
-                    for (int p = 0; p < PH; ++p)
-                        hv[q][t][p] = ok && live[t] ? *reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(a.h) + (p * a.h_plane + h[t] + kq) * W::SZ)
-                                                    : make_uint4(0u, 0u, 0u, 0u);
+            for (int t = 0; t < MT; ++t) {
+                live[t] = m0 + t * 16 + r16 < count;
+                entry[t] = live[t] ? row_of_table[2 + m0 + t * 16 + r16] : 0;
+                wt[t] = a.wts[entry[t]];
+                h[t] = (int64_t)entry[t] * a.inter + g * CE;
             }
+            f32x4_t acc[MT];
 #pragma unroll
-            for (int q = 0; q < 2 * U; ++q) {
-                uint4 pw[W::PARTS];
-                if constexpr (P != P_F32) w[q].parts(pw);
+            for (int t = 0; t < MT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            constexpr int U = W::RAW + MT * PH > 4 ? 1 : W::RAW + MT * PH > 2 ? 2 : 4;    // pieces in flight a wave, by registers
+            const int K = k_hi - g * CE;
+            for (int k = k_lo + wave * PIECE; k < k_hi; k += U * WAVES * PIECE) {
+                W w[2 * U];
+                uint4 hv[2 * U][MT][PH];
 #pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    if constexpr (P == P_F32) acc[t] = mfma_f(w[q].raw[0], hv[q][t][0], acc[t]);
-                    else acc[t] = mfma_parts<W::PARTS, PH, PH>(pw, hv[q][t], acc[t]);
+                for (int q = 0; q < 2 * U; ++q) {
+                    const int kq = k + (q >> 1) * WAVES * PIECE + (q & 1) * 4 * CE;
+                    const bool ok = kq < K;
+                    if (ok) w[q].load(a.w2, row + kq, low);
+                    else w[q].clear();
+#pragma unroll
+                    for (int t = 0; t < MT; ++t)
+#pragma unroll
+                        for (int p = 0; p < PH; ++p)
+                            hv[q][t][p] = ok && live[t] ? *reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(a.h) + (p * a.h_plane + h[t] + kq) * W::SZ)
+                                                        : make_uint4(0u, 0u, 0u, 0u);
+                }
+#pragma unroll
+                for (int q = 0; q < 2 * U; ++q) {
+                    uint4 pw[W::PARTS];
+                    if constexpr (P != P_F32) w[q].parts(pw);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        if constexpr (P == P_F32) acc[t] = mfma_f(w[q].raw[0], hv[q][t][0], acc[t]);
+                        else acc[t] = mfma_parts<W::PARTS, PH, PH>(pw, hv[q][t], acc[t]);
+                    }
                 }
             }
+            // a token chooses an expert once: the lanes of a wave add to different rows
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                if (live[t]) {
+                    const int tok = entry[t] / a.top_k;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) ysum[wave][tok][4 * g + q] += wt[t] * acc[t][q];
+                }
         }
-        // a token chooses an expert once: the lanes of a wave add to different rows
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-            if (live[t]) {
-                const int en = ch.entry[t * 16 + r16], tok = en / a.top_k;
-                const float wt = wts_s[en];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) ysum[wave][tok][4 * g + q] += wt * acc[t][q];
-            }
     }
     __syncthreads();
     const A* res = static_cast<const A*>(a.res);
@@ -419,22 +466,28 @@ __global__ __launch_bounds__(64 * WAVES) void few_down_kernel(const FewArgs a) {
         float v = 0.f;
 #pragma unroll
         for (int s = 0; s < WAVES; ++s) v += ysum[s][t][c];
-        a.part[((int64_t)blockIdx.y * a.T + t) * a.d + col0 + c] = v;
+        __hip_atomic_store(&a.part[((int64_t)blockIdx.y * a.T + t) * a.d + col0 + c], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    // The last workgroup of this column group adds the shares.  Nobody waits: the others have left.  Release: every wave's shares are
-    // visible to the device before the count; acquire: the last one reads what all counted workgroups wrote.
-    __threadfence();
+    // The last workgroup of this column group adds the shares.  Nobody waits: the others have left.  The shares are written and read
+    // by device-scope accesses, which go past the L2 of an XCD; every wave waits for its own to arrive before the workgroup is counted.
+    // (A device-scope fence does the same by writing back the whole L2: 40 us for one token of width 512.)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (tid == 0) last = __hip_atomic_fetch_add(&a.arrived[blockIdx.x], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.shares - 1;
+    if (tid == 0) last = __hip_atomic_fetch_add(&a.arrived[blockIdx.x], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.shares - 1;
     __syncthreads();
     if (!last) return;
-    __threadfence();
     for (int i = tid; i < a.T * 16; i += 64 * WAVES) {
         const int t = i >> 4, c = i & 15;
         const int64_t at = (int64_t)t * a.d + col0 + c;
         float v = res ? (float)res[at] : 0.f;
         float s = 0.f;
-        for (int p = 0; p < a.shares; ++p) s += a.part[(int64_t)p * a.T * a.d + at];
+        for (int p0 = 0; p0 < a.shares; p0 += 8) {                        // eight loads in flight, added in order
+            float f[8];
+#pragma unroll
+            for (int p = 0; p < 8; ++p) f[p] = __hip_atomic_load(&a.part[(int64_t)min(p0 + p, a.shares - 1) * a.T * a.d + at], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+            for (int p = 0; p < 8; ++p) s += p0 + p < a.shares ? f[p] : 0.f;
+        }
         y[at] = (A)(s + v);
     }
 }
@@ -442,7 +495,7 @@ __global__ __launch_bounds__(64 * WAVES) void few_down_kernel(const FewArgs a) {
 // ------------------------------------------------------------------------------------------------------------- host
 inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-struct FewPlan { int shares, k_splits, active; size_t idx, wts, h, part, arrived, bytes; int64_t h_plane; };
+struct FewPlan { int shares, k_splits, active; size_t idx, wts, table, h, part, arrived, bytes; int64_t h_plane; };
 
 FewPlan few_plan(int T, int d, int inter, int E, int top_k, int act_type, int precision) {
     FewPlan p;
@@ -455,12 +508,15 @@ FewPlan few_plan(int T, int d, int inter, int E, int top_k, int act_type, int pr
     p.k_splits = 1;
     if (want > p.active) p.k_splits = (want + p.active - 1) / p.active;
     if (p.k_splits > most_k) p.k_splits = most_k;
-    p.shares = p.active * p.k_splits < want ? p.active * p.k_splits : want;
+    // as many units each: an uneven share is a second round for all
+    const int units = p.active * p.k_splits, per = units > want ? units / want : 1;
+    p.shares = (units + per - 1) / per;
     p.h_plane = (int64_t)n * inter;
     size_t off = 0;
     auto take = [&](size_t b) { const size_t at = off; off += up256(b); return at; };
     p.idx = take((size_t)n * 4);
     p.wts = take((size_t)n * 4);
+    p.table = take((size_t)p.active * (T + 2) * 4);
     p.h = take((size_t)p.h_plane * (precision == P_F32 ? 4 : act_type == DT_F32 ? 6 : 4));
     p.part = take(p.shares > 1 ? (size_t)p.shares * T * d * 4 : 0);
     p.arrived = take((size_t)groups * 4);
@@ -478,10 +534,14 @@ bool few_types_ok(int act_type, int precision) {
     return (act_type == DT_BF16 && precision == P_BF16) || (act_type == DT_F16 && precision == P_F16);
 }
 
+// tokens times groups of eight experts up to which `up` routes by itself
+constexpr int ROUTE_INSIDE = 2;
+static_assert(ROUTE_INSIDE <= ROUTE_GROUPS, "fits LDS");
+
 template <typename A, int P, int MT>
 void launch_few_layer(const FewArgs& a, const FewPlan& p, hipStream_t s) {
     const dim3 up((unsigned)(a.inter / 16), (unsigned)p.active), down((unsigned)(a.d / 16), (unsigned)p.shares), block(64 * WAVES);
-    if ((int64_t)a.T * a.E * a.d <= ROUTE_INSIDE) {
+    if (a.T * ((a.E + 7) / 8) <= ROUTE_INSIDE) {
         hipLaunchKernelGGL((few_up_kernel<A, P, MT, true>), up, block, 0, s, a);
     } else {
         hipLaunchKernelGGL(few_route_kernel<A>, dim3((unsigned)a.T), block, 0, s, a);
@@ -493,8 +553,7 @@ void launch_few_layer(const FewArgs& a, const FewPlan& p, hipStream_t s) {
 template <typename A, int P>
 void launch_by_tokens(const FewArgs& a, const FewPlan& p, hipStream_t s) {
     if (a.T <= 16) launch_few_layer<A, P, 1>(a, p, s);
-    else if (a.T <= 32) launch_few_layer<A, P, 2>(a, p, s);
-    else launch_few_layer<A, P, 4>(a, p, s);
+    else launch_few_layer<A, P, 2>(a, p, s);
 }
 
 }  // namespace
@@ -528,6 +587,7 @@ ADX_API int adx_op_moe_few(const void* x, const void* res, const float* router_w
     FewArgs a;
     a.x = x; a.res = res; a.router = router_w; a.w13 = w13; a.w2 = w2; a.T = T; a.d = d; a.inter = inter; a.E = E; a.top_k = top_k;
     a.idx = reinterpret_cast<int*>(base + p.idx); a.wts = reinterpret_cast<float*>(base + p.wts);
+    a.table = reinterpret_cast<int*>(base + p.table); a.active = p.active;
     a.h = base + p.h; a.h_plane = p.h_plane; a.part = reinterpret_cast<float*>(base + p.part); a.arrived = reinterpret_cast<int*>(base + p.arrived);
     a.shares = p.shares; a.k_splits = p.k_splits; a.y = y;
     hipStream_t s = (hipStream_t)stream;

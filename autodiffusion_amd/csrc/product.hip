@@ -5,6 +5,7 @@
 // operands.  Sums are fp32; bias, activation and residual are applied to the fp32 sum and the result is rounded once.
 #include "adx_ops.h"
 #include "engine.h"
+#include "fastmath.h"
 #include "typed.h"
 
 #include <type_traits>
@@ -17,6 +18,23 @@ constexpr int ACT_TANH_ = 6;
 __device__ __align__(16) unsigned char zero_chunk[16];            // what copies past the end of the summed axis read
 
 // ------------------------------------------------------------------------------------------------------------- activations
+// erfc(u) / 2 for u >= 0, times exp(u^2): a polynomial in 1 / (1 + u / 2) (the Chebyshev fit of the textbooks, fractional error 1.2e-7:
+// two fp32 roundings, also in the tail, where 1 - erf has none left).  A quarter of the instructions of erff.
+__device__ __forceinline__ float half_erfc_scaled_log(float t) {
+    float p = 0.17087277f;
+    p = p * t - 0.82215223f; p = p * t + 1.48851587f; p = p * t - 1.13520398f; p = p * t + 0.27886807f; p = p * t - 0.18628806f;
+    p = p * t + 0.09678418f; p = p * t + 0.37409196f; p = p * t + 1.00002368f;
+    return p * t - 1.26551223f;
+}
+// Phi(-|z|), the smaller tail of the normal distribution
+__device__ __forceinline__ float normal_tail(float z) {
+    const float u = fabsf(z) * 0.70710678118654752f, t = rcp_fast(1.f + 0.5f * u);
+    return 0.5f * t * exp2_fast((half_erfc_scaled_log(t) - u * u) * 1.44269504088896341f);
+}
+__device__ __forceinline__ float sigmoid_fast(float z) { return rcp_fast(1.f + exp2_fast(-1.44269504088896341f * z)); }
+// z + 0.044715 z^3 scaled so that its sigmoid is (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2
+__device__ __forceinline__ float gelu_tanh_arg(float z) { return 1.59576912160573071f * z * (1.f + 0.044715f * z * z); }
+
 template <int V> __device__ __forceinline__ void apply_act(float (&v)[V], int act) {
     switch (act) {                                                 // uniform: one branch for all values
         case ACT_RELU:
@@ -29,7 +47,7 @@ template <int V> __device__ __forceinline__ void apply_act(float (&v)[V], int ac
             break;
         case ACT_SILU:
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = v[e] / (1.f + expf(-v[e]));
+            for (int e = 0; e < V; ++e) v[e] *= sigmoid_fast(v[e]);
             break;
         case ACT_TANH_:
 #pragma unroll
@@ -37,28 +55,52 @@ template <int V> __device__ __forceinline__ void apply_act(float (&v)[V], int ac
             break;
         case ACT_GELU_ERF:
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = 0.5f * v[e] * (1.f + erff(v[e] * 0.70710678118654752f));
+            for (int e = 0; e < V; ++e) { const float q = normal_tail(v[e]); v[e] *= v[e] > 0.f ? 1.f - q : q; }
             break;
         case ACT_GELU_TANH:
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = 0.5f * v[e] * (1.f + tanhf(0.79788456080286536f * (v[e] + 0.044715f * v[e] * v[e] * v[e])));
+            for (int e = 0; e < V; ++e) v[e] *= sigmoid_fast(gelu_tanh_arg(v[e]));
             break;
         default: break;
     }
 }
 
-__device__ __forceinline__ float act_slope(float z, int act) {
+template <int V> __device__ __forceinline__ void act_slopes(const float (&z)[V], float (&d)[V], int act) {
     switch (act) {
-        case ACT_RELU: return z > 0.f ? 1.f : 0.f;
-        case ACT_LEAKY: return z > 0.f ? 1.f : 0.01f;
-        case ACT_SILU: { const float g = 1.f / (1.f + expf(-z)); return g * (1.f + z * (1.f - g)); }
-        case ACT_TANH_: { const float t = tanhf(z); return 1.f - t * t; }
-        case ACT_GELU_ERF: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
-        case ACT_GELU_TANH: {
-            const float t = tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z));
-            return 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * 0.79788456080286536f * (1.f + 0.134145f * z * z);
-        }
-        default: return 1.f;
+        case ACT_RELU:
+#pragma unroll
+            for (int e = 0; e < V; ++e) d[e] = z[e] > 0.f ? 1.f : 0.f;
+            break;
+        case ACT_LEAKY:
+#pragma unroll
+            for (int e = 0; e < V; ++e) d[e] = z[e] > 0.f ? 1.f : 0.01f;
+            break;
+        case ACT_SILU:
+#pragma unroll
+            for (int e = 0; e < V; ++e) { const float g = sigmoid_fast(z[e]); d[e] = g * (1.f + z[e] * (1.f - g)); }
+            break;
+        case ACT_TANH_:
+#pragma unroll
+            for (int e = 0; e < V; ++e) { const float t = tanhf(z[e]); d[e] = 1.f - t * t; }
+            break;
+        case ACT_GELU_ERF:
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float q = normal_tail(z[e]);
+                d[e] = (z[e] > 0.f ? 1.f - q : q) + z[e] * 0.39894228040143268f * exp2_fast(-0.72134752044448170f * z[e] * z[e]);
+            }
+            break;
+        case ACT_GELU_TANH:
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float c = fminf(fmaxf(z[e], -30.f), 30.f), g = sigmoid_fast(gelu_tanh_arg(c));      // beyond 30 the slope is 0 or 1
+                d[e] = g + c * g * (1.f - g) * 1.59576912160573071f * (1.f + 0.134145f * c * c);
+                if (z[e] != z[e]) d[e] = z[e];
+            }
+            break;
+        default:
+#pragma unroll
+            for (int e = 0; e < V; ++e) d[e] = 1.f;
     }
 }
 
@@ -124,15 +166,20 @@ __device__ __forceinline__ void finish(const ProductArgs& a, int64_t m, int n, f
 }
 
 // ------------------------------------------------------------------------------------------------------------- large tiles
-typedef const __attribute__((address_space(3))) void* lds_cptr;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
 // 64 x 16 bytes from per-lane global addresses to 1 KB of LDS.  Issued from inline assembly: the compiler would make every later LDS
 // read wait for all copies it knows of; the kernel orders them itself with counted waits and barriers.
-__device__ __forceinline__ void copy_1k(const void* g, unsigned lds_uniform) {
+__device__ __forceinline__ void copy_1k_lanes(const void* g, unsigned lds_uniform) {
     unsigned keep;          // m0 is restored: the compiler does not expect inline assembly to change it
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep) : "s"(lds_uniform), "v"(g) : "memory");
+}
+// the same with a wave-uniform base and a 32-bit byte offset a lane: no vector arithmetic
+__device__ __forceinline__ void copy_1k(const void* base_uniform, unsigned lane_offset, unsigned lds_uniform) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "s"(lds_uniform), "v"(lane_offset), "s"(base_uniform) : "memory");
 }
 template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -142,14 +189,15 @@ __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
 }
 
-// One operand's part of a tile: ROWS of its own index x 128 bytes of k, in one of two LDS images.
-//   row:    [ROWS][128 B]; 16-byte chunk c of row r sits at c ^ ((r >> 1) & 7): the fragment read (32 rows x one chunk) meets
+// One operand's part of a K step: ROWS of its own index x 64 bytes of k, an image in LDS.
+//   row:    [ROWS][64 B]; 16-byte chunk c of row r sits at c ^ ((r >> 2) & 3): 16 rows of one chunk (a quarter of a fragment read) meet
 //           every bank once
 //   column: [KE][ROWS]; the 16-bit fragment read is the transposing LDS read (4 k-rows x 16 own indices a 16-lane group): 32-byte unit
 //           u of k-row k sits at u ^ f(k) so that the k-rows of one read lie in different banks; fp32 reads 32 consecutive values
-template <typename T, bool COL, int ROWS> struct Side {
-    static constexpr int SZ = sizeof(T), CE = 16 / SZ, KE = 128 / SZ;
-    static constexpr int BYTES = ROWS * 128, SLABS = BYTES / 1024, RB = ROWS * SZ;
+template <typename T, bool COL, int ROWS, int KB> struct Side {
+    static constexpr int SZ = sizeof(T), CE = 16 / SZ, KE = KB / SZ;
+    static constexpr int BYTES = ROWS * KB, SLABS = BYTES / 1024, RB = ROWS * SZ;
+    static __device__ __forceinline__ int row_swizzle(int r) { return KB == 64 ? (r >> 2) & 3 : (r >> 1) & 7; }
     static __device__ __forceinline__ int unit_swizzle(int k) {
         if constexpr (SZ == 2) { constexpr int mask = RB / 32 - 1; return (((k & 3) | (((k >> 3) & 1) << 2)) & mask) << 5; }
         else return ((k >> 2) & 1) << 7;
@@ -157,8 +205,9 @@ template <typename T, bool COL, int ROWS> struct Side {
     // own index and first k (relative to the tile) of the 16 bytes that lane `lane` copies to slab `slab`
     static __device__ __forceinline__ void source(int slab, int lane, int& row, int& k) {
         if constexpr (!COL) {
-            row = slab * 8 + (lane >> 3);
-            k = ((lane & 7) ^ ((row >> 1) & 7)) * CE;
+            constexpr int CPR = KB / 16;                       // chunks of a row
+            row = slab * (64 / CPR) + lane / CPR;
+            k = ((lane & (CPR - 1)) ^ row_swizzle(row)) * CE;
         } else {
             const int at = slab * 1024 + lane * 16;
             k = at / RB;
@@ -169,7 +218,7 @@ template <typename T, bool COL, int ROWS> struct Side {
     static __device__ __forceinline__ uint4 fragment(const unsigned char* img, int base, int kk, int lane) {
         if constexpr (!COL) {
             const int r = base + (lane & 31), c = 2 * kk + (lane >> 5);
-            return *reinterpret_cast<const uint4*>(img + r * 128 + ((c ^ ((r >> 1) & 7)) << 4));
+            return *reinterpret_cast<const uint4*>(img + r * KB + ((c ^ row_swizzle(r)) << 4));
         } else if constexpr (SZ == 2) {
             typedef short s4 __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) s4* s4p;
@@ -203,128 +252,13 @@ template <typename T> __device__ __forceinline__ f32x16_t mfma32(const uint4& a,
     }
 }
 
-// Workgroup tile BM x BN, WM x WN waves, a K step of 128 bytes a row, two LDS slots.  DMA: copies from global memory straight to
-// LDS (operands whose rows start on 16 bytes); otherwise element loads through registers into the same images.
-template <typename T, bool ACOL, bool BCOL, int BM, int BN, int WM, int WN, bool DMA>
-__global__ __launch_bounds__(64 * WM * WN) void product_kernel(const ProductArgs a) {
-    typedef Side<T, ACOL, BM> SA;
-    typedef Side<T, BCOL, BN> SB;
-    constexpr int W = WM * WN, KE = SA::KE, CE = SA::CE, SZ = sizeof(T);
-    constexpr int FI = BM / WM / 32, FJ = BN / WN / 32, NW = BN / WN;
-    constexpr int SLOT = SA::BYTES + SB::BYTES, PA = SA::SLABS / W, PB = SB::SLABS / W;
-    constexpr int EP_LD = NW + 4;
-    static_assert(SA::SLABS % W == 0 && SB::SLABS % W == 0, "slabs spread evenly over the waves");
-    static_assert(W * 32 * EP_LD * 4 <= 2 * SLOT, "the epilogue's patches fit the slots");
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SLOT];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // XCD x (blockIdx % 8) walks a contiguous range of an order of column panels eight tiles wide, so that the workgroups that
-    // run on an XCD at one time share rows and columns in its L2
-    const int n_tiles = a.tiles_m * a.tiles_n, per_xcd = (n_tiles + 7) / 8;
-    const int lin = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-    if (lin >= n_tiles) return;
-    const int panel = lin / (a.tiles_m * 8), width = min(8, a.tiles_n - panel * 8), in = lin - panel * a.tiles_m * 8;
-    const int64_t m0 = (int64_t)(in / width) * BM;
-    const int n0 = (panel * 8 + in % width) * BN;
-    const int64_t k_lo = (int64_t)blockIdx.y * a.k_split, k_hi = k_lo + a.k_split < a.K ? k_lo + a.k_split : a.K;
-    const int nk = (int)((k_hi - k_lo + KE - 1) / KE);
-    const int wm = wave / WN, wn = wave % WN;
-
-    const unsigned lds0 = (unsigned)(uintptr_t)(lds_ptr)smem;
-    const unsigned char *pa[PA], *pb[PB];                     // this lane's source of its slabs, K step 0
-    int ka[PA], kb[PB];                                        // its k relative to the step
-    int64_t ra[PA], rb[PB];
-#pragma unroll
-    for (int i = 0; i < PA; ++i) {
-        int row;
-        SA::source(wave + i * W, lane, row, ka[i]);
-        ra[i] = m0 + row;
-        // a row image repeats its last row past the end (those results are not stored); a column image has chunks past the end,
-        // which are not read
-        if constexpr (!ACOL) { if (ra[i] > a.M - 1) ra[i] = a.M - 1; }
-        pa[i] = static_cast<const unsigned char*>(a.A) + (ACOL ? (k_lo + ka[i]) * a.lda + ra[i] : ra[i] * a.lda + k_lo + ka[i]) * SZ;
-        if (ACOL && ra[i] >= a.M) ka[i] = 1 << 30;
-    }
-#pragma unroll
-    for (int i = 0; i < PB; ++i) {
-        int row;
-        SB::source(wave + i * W, lane, row, kb[i]);
-        rb[i] = n0 + row;
-        if constexpr (!BCOL) { if (rb[i] > a.N - 1) rb[i] = a.N - 1; }
-        pb[i] = static_cast<const unsigned char*>(a.B) + (BCOL ? (k_lo + kb[i]) * a.ldb + rb[i] : rb[i] * a.ldb + k_lo + kb[i]) * SZ;
-        if (BCOL && rb[i] >= a.N) kb[i] = 1 << 30;
-    }
-    const int64_t step_a = (ACOL ? a.lda * KE : KE) * SZ, step_b = (BCOL ? a.ldb * KE : KE) * SZ;
-    auto issue = [&](int kt) {                                 // K step kt -> slot kt & 1; what lies past the end is zero
-        const unsigned slot = (unsigned)(kt & 1) * SLOT;
-        const int left = (int)(k_hi - k_lo < (int64_t)(kt + 1) * KE ? k_hi - k_lo - (int64_t)kt * KE : KE);      // valid k of this step (<= 0 past the end)
-        if constexpr (DMA) {
-#pragma unroll
-            for (int i = 0; i < PA; ++i) {
-                copy_1k(ka[i] < left ? pa[i] : zero_chunk, lds0 + slot + (unsigned)(wave + i * W) * 1024u);
-                pa[i] += step_a;
-            }
-#pragma unroll
-            for (int i = 0; i < PB; ++i) {
-                copy_1k(kb[i] < left ? pb[i] : zero_chunk, lds0 + slot + SA::BYTES + (unsigned)(wave + i * W) * 1024u);
-                pb[i] += step_b;
-            }
-        } else {
-            auto gather = [&](const unsigned char* p, int k, int64_t own, int64_t own_end, bool col, unsigned at) {
-                T v[CE];
-#pragma unroll
-                for (int e = 0; e < CE; ++e) {
-                    const bool ok = col ? (k < left && own + e < own_end) : (k + e < left);
-                    v[e] = ok ? reinterpret_cast<const T*>(p)[e] : (T)0.f;
-                }
-                *reinterpret_cast<Pack<T, CE>*>(smem + at + lane * 16) = *reinterpret_cast<Pack<T, CE>*>(v);
-            };
-#pragma unroll
-            for (int i = 0; i < PA; ++i) { gather(pa[i], ka[i], ra[i], a.M, ACOL, slot + (wave + i * W) * 1024); pa[i] += step_a; }
-#pragma unroll
-            for (int i = 0; i < PB; ++i) { gather(pb[i], kb[i], rb[i], a.N, BCOL, slot + SA::BYTES + (wave + i * W) * 1024); pb[i] += step_b; }
-        }
-    };
-
-    f32x16_t acc[FI][FJ];
-#pragma unroll
-    for (int i = 0; i < FI; ++i)
-#pragma unroll
-        for (int j = 0; j < FJ; ++j)
-#pragma unroll
-            for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
-
-    issue(0);
-    issue(1);
-    for (int kt = 0; kt < nk; ++kt) {
-        wait_copies<PA + PB>();                                // this wave's copies of step kt have landed ...
-        if constexpr (!DMA) wait_lds();
-        barrier();                                             // ... and everybody's
-        const unsigned char* img = smem + (kt & 1) * SLOT;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            uint4 fa[FI], fb[FJ];
-#pragma unroll
-            for (int j = 0; j < FJ; ++j) fb[j] = SB::fragment(img + SA::BYTES, wn * NW + j * 32, kk, lane);
-#pragma unroll
-            for (int i = 0; i < FI; ++i) fa[i] = SA::fragment(img, wm * (BM / WM) + i * 32, kk, lane);
-#pragma unroll
-            for (int i = 0; i < FI; ++i)
-#pragma unroll
-                for (int j = 0; j < FJ; ++j) acc[i][j] = mfma32<T>(fb[j], fa[i], acc[i][j]);      // rows of the result: n; columns: m
-        }
-        wait_lds();
-        barrier();                                             // nobody reads the slot any more
-        issue(kt + 2);
-    }
-    wait_copies<0>();
-    if constexpr (!DMA) wait_lds();
-    barrier();
-
-    // Epilogue: 32 rows x NW columns at a time through LDS, so that a row's columns are stored as whole lines.  Result layout of the
-    // 32x32 product: column = lane & 31, row = (q & 3) + 8 (q >> 2) + 4 (lane >> 5).
-    constexpr int V = 16 / SZ, LPR = NW / V, RPI = 64 / LPR;   // lanes of a row, rows of one pass
+// Epilogue of a wave's 32 FI x 32 FJ results: 32 rows at a time through LDS, so that a row's columns are stored as whole lines.
+// Result layout of the 32x32 product: column = lane & 31, row = (q & 3) + 8 (q >> 2) + 4 (lane >> 5).
+template <typename T, int FI, int FJ>
+__device__ __forceinline__ void store_tile(const ProductArgs& a, f32x16_t (&acc)[FI][FJ], unsigned char* smem, int64_t m_wave, int n_wave, int wave, int lane) {
+    constexpr int NW = FJ * 32, EP_LD = NW + 4, V = 16 / sizeof(T), LPR = NW / V, RPI = 64 / LPR;   // lanes of a row, rows of one pass
     float* patch = reinterpret_cast<float*>(smem) + wave * 32 * EP_LD;
-    const int n = n0 + wn * NW + (lane % LPR) * V;
+    const int n = n_wave + (lane % LPR) * V;
 #pragma unroll
     for (int i = 0; i < FI; ++i) {
         __builtin_amdgcn_wave_barrier();
@@ -339,7 +273,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const ProductArgs
 #pragma unroll 1
         for (int p = 0; p < 32 / RPI; ++p) {
             const int r = p * RPI + lane / LPR;
-            const int64_t m = m0 + wm * (BM / WM) + i * 32 + r;
+            const int64_t m = m_wave + i * 32 + r;
             float v[V];
 #pragma unroll
             for (int e = 0; e < V; e += 4) {
@@ -361,6 +295,179 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(const ProductArgs
         }
         wait_lds();
     }
+}
+
+// Workgroup tile BM x BN, WM x WN waves, a K step of KB bytes a row, a ring of R LDS slots.  Copies go straight from global memory to
+// LDS and are R - 1 steps ahead.  One barrier a step: a wave passes it when it holds the step's last fragments in registers and
+// its copies of the next step have landed; behind it the step's slot is refilled and the next step is read, both under the step's
+// last products.  Fragments are read under the products before theirs, all of them in front of the first half of those.
+template <typename T, bool ACOL, bool BCOL, int BM, int BN, int WM, int WN, int KB, int R>
+__global__ __launch_bounds__(64 * WM * WN, 2) void product_kernel(const ProductArgs a) {
+    typedef Side<T, ACOL, BM, KB> SA;
+    typedef Side<T, BCOL, BN, KB> SB;
+    constexpr int W = WM * WN, KE = SA::KE, SZ = sizeof(T);
+    constexpr int FI = BM / WM / 32, FJ = BN / WN / 32, NW = BN / WN, NKK = KB / 32;
+    constexpr int SLOT = SA::BYTES + SB::BYTES, PA = SA::SLABS / W, PB = SB::SLABS / W, P = PA + PB;
+    constexpr int EP_LD = NW + 4;
+    static_assert(SA::SLABS % W == 0 && SB::SLABS % W == 0, "slabs spread evenly over the waves");
+    static_assert(W * 32 * EP_LD * 4 <= R * SLOT, "the epilogue's patches fit the slots");
+    static_assert((R & (R - 1)) == 0 && (R - 1) * P < 64, "slot of a step by mask; counted waits");
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[R * SLOT];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // XCD x (blockIdx % 8) walks a contiguous range of an order of column panels eight tiles wide, so that the workgroups that
+    // run on an XCD at one time share rows and columns in its L2
+    const int n_tiles = a.tiles_m * a.tiles_n, per_xcd = (n_tiles + 7) / 8;
+    const int lin = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+    if (lin >= n_tiles) return;
+    const int panel = lin / (a.tiles_m * 8), width = min(8, a.tiles_n - panel * 8), in = lin - panel * a.tiles_m * 8;
+    const int64_t m0 = (int64_t)(in / width) * BM;
+    const int n0 = (panel * 8 + in % width) * BN;
+    const int64_t k_lo = (int64_t)blockIdx.y * a.k_split, k_len = (k_lo + a.k_split < a.K ? k_lo + a.k_split : a.K) - k_lo;
+    const int nk = (int)((k_len + KE - 1) / KE);
+    const int wm = wave / WN, wn = wave % WN;
+
+    // Sources: a wave-uniform base that advances by a step, a constant 32-bit byte offset a lane (the host checks that tiles span less
+    // than 2^31 bytes).  Own indices past the end repeat the last valid ones (those results are not stored); k past the end reads zeros.
+    const unsigned lds0 = (unsigned)(uintptr_t)(lds_ptr)smem;
+    unsigned oa[PA], ob[PB];
+    int ka[PA], kb[PB];
+    const int64_t row_end = a.M - m0, col_end = a.N - n0;
+#pragma unroll
+    for (int i = 0; i < PA; ++i) {
+        int row;
+        SA::source(wave + i * W, lane, row, ka[i]);
+        const int last = (int)(row_end < BM ? row_end : BM) - (ACOL ? SA::CE : 1);
+        row = min(row, last);
+        oa[i] = (unsigned)((ACOL ? (int64_t)ka[i] * a.lda + row : (int64_t)row * a.lda + ka[i]) * SZ);
+    }
+#pragma unroll
+    for (int i = 0; i < PB; ++i) {
+        int row;
+        SB::source(wave + i * W, lane, row, kb[i]);
+        const int last = (int)(col_end < BN ? col_end : BN) - (BCOL ? SB::CE : 1);
+        row = min(row, last);
+        ob[i] = (unsigned)((BCOL ? (int64_t)kb[i] * a.ldb + row : (int64_t)row * a.ldb + kb[i]) * SZ);
+    }
+    const unsigned char* base_a = static_cast<const unsigned char*>(a.A) + (ACOL ? k_lo * a.lda + m0 : m0 * a.lda + k_lo) * SZ;
+    const unsigned char* base_b = static_cast<const unsigned char*>(a.B) + (BCOL ? k_lo * a.ldb + n0 : (int64_t)n0 * a.ldb + k_lo) * SZ;
+    const int64_t step_a = (ACOL ? a.lda * KE : KE) * SZ, step_b = (BCOL ? a.ldb * KE : KE) * SZ;
+    int left = (int)k_len;                                     // valid k from the next step to copy on
+    // the i-th of this wave's copies of the next step, into its slot
+    auto copy_a = [&](int i, unsigned slot) {
+        const unsigned at = lds0 + slot + (unsigned)(wave + i * W) * 1024u;
+        if (left >= KE) copy_1k(base_a, oa[i], at);
+        else copy_1k_lanes(ka[i] < left ? base_a + oa[i] : zero_chunk, at);
+    };
+    auto copy_b = [&](int i, unsigned slot) {
+        const unsigned at = lds0 + slot + SA::BYTES + (unsigned)(wave + i * W) * 1024u;
+        if (left >= KE) copy_1k(base_b, ob[i], at);
+        else copy_1k_lanes(kb[i] < left ? base_b + ob[i] : zero_chunk, at);
+    };
+    auto advance = [&]() { base_a += step_a; base_b += step_b; left -= KE; };
+
+    f32x16_t acc[FI][FJ];
+#pragma unroll
+    for (int i = 0; i < FI; ++i)
+#pragma unroll
+        for (int j = 0; j < FJ; ++j)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
+
+#pragma unroll
+    for (int t = 0; t < R; ++t) {
+#pragma unroll
+        for (int i = 0; i < PA; ++i) copy_a(i, t * SLOT);
+#pragma unroll
+        for (int i = 0; i < PB; ++i) copy_b(i, t * SLOT);
+        advance();
+    }
+    wait_copies<(R - 1) * P>();
+    barrier();
+    uint4 fa[2][FI], fb[2][FJ];
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) fb[0][j] = SB::fragment(smem + SA::BYTES, wn * NW + j * 32, 0, lane);
+#pragma unroll
+    for (int i = 0; i < FI; ++i) fa[0][i] = SA::fragment(smem, wm * (BM / WM) + i * 32, 0, lane);
+    for (int kt = 0; kt < nk; ++kt) {
+        const unsigned slot = (unsigned)(kt & (R - 1)) * SLOT, next = (unsigned)((kt + 1) & (R - 1)) * SLOT;
+#pragma unroll
+        for (int kk = 0; kk < NKK; ++kk) {
+            const bool turn = kk == NKK - 1;
+            if (turn) {
+                wait_lds();                                    // this wave has read all of the step ...
+                wait_copies<(R - 2) * P>();                    // ... and its copies of the next one have landed
+                barrier();
+            }
+            const unsigned char* img = smem + (turn ? next : slot);
+            const int to = (kk + 1) & 1, at = turn ? 0 : kk + 1;
+#pragma unroll
+            for (int i = 0; i < FI; ++i) {
+                if (i == 0) {
+#pragma unroll
+                    for (int j = 0; j < FJ; ++j) fb[to][j] = SB::fragment(img + SA::BYTES, wn * NW + j * 32, at, lane);
+                }
+                if (2 * i < FI) {
+#pragma unroll
+                    for (int r = 2 * i; r < min(2 * i + 2, FI); ++r) fa[to][r] = SA::fragment(img, wm * (BM / WM) + r * 32, at, lane);
+                }
+                if (turn) {
+#pragma unroll
+                    for (int p = i * PA / FI; p < (i + 1) * PA / FI; ++p) copy_a(p, slot);
+#pragma unroll
+                    for (int p = i * PB / FI; p < (i + 1) * PB / FI; ++p) copy_b(p, slot);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < FJ; ++j) acc[i][j] = mfma32<T>(fb[kk & 1][j], fa[kk & 1][i], acc[i][j]);      // rows of the result: n; columns: m
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        advance();
+    }
+    wait_copies<0>();
+    wait_lds();
+    barrier();
+
+    store_tile<T, FI, FJ>(a, acc, smem, m0 + wm * (BM / WM), n0 + wn * NW, wave, lane);
+}
+
+// Operands whose rows start on no 16 bytes: element loads through registers into the same images, 64 x 64 tiles, one slot.
+template <typename T, bool ACOL, bool BCOL>
+__global__ __launch_bounds__(256) void product_any_kernel(const ProductArgs a) {
+    typedef Side<T, ACOL, 64, 64> SA;
+    typedef Side<T, BCOL, 64, 64> SB;
+    constexpr int KE = SA::KE, CE = SA::CE;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * 32 * 36 * 4];             // two images, then the epilogue's patches
+    static_assert(sizeof(smem) >= SA::BYTES + SB::BYTES, "images fit");
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
+    const int64_t m0 = (int64_t)(blockIdx.x / a.tiles_n) * 64;
+    const int n0 = (int)(blockIdx.x % a.tiles_n) * 64;
+    const int64_t k_lo = (int64_t)blockIdx.y * a.k_split, k_hi = k_lo + a.k_split < a.K ? k_lo + a.k_split : a.K;
+    auto gather = [&](const void* base, int64_t ld, bool col, int64_t own, int64_t own_end, int64_t k, unsigned at) {
+        Pack<T, CE> v;
+#pragma unroll
+        for (int e = 0; e < CE; ++e) {
+            const int64_t o = col ? own + e : own, kk = col ? k : k + e;
+            v.v[e] = o < own_end && kk < k_hi ? static_cast<const T*>(base)[col ? kk * ld + o : o * ld + kk] : (T)0.f;
+        }
+        *reinterpret_cast<Pack<T, CE>*>(smem + at) = v;
+    };
+    f32x16_t acc[1][1];
+#pragma unroll
+    for (int q = 0; q < 16; ++q) acc[0][0][q] = 0.f;
+    int ra, ka, rb, kb;
+    SA::source(wave, lane, ra, ka);
+    SB::source(wave, lane, rb, kb);
+    for (int64_t k = k_lo; k < k_hi; k += KE) {
+        gather(a.A, a.lda, ACOL, m0 + ra, a.M, k + ka, tid * 16);
+        gather(a.B, a.ldb, BCOL, n0 + rb, a.N, k + kb, SA::BYTES + tid * 16);
+        __syncthreads();
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+            acc[0][0] = mfma32<T>(SB::fragment(smem + SA::BYTES, wn * 32, kk, lane), SA::fragment(smem, wm * 32, kk, lane), acc[0][0]);
+        __syncthreads();
+    }
+    store_tile<T, 1, 1>(a, acc, smem, m0 + wm * 32, n0 + wn * 32, wave, lane);
 }
 
 // the partial sums of a split product, added in split order, and the epilogue
@@ -500,9 +607,13 @@ __global__ __launch_bounds__(256) void slope_kernel(const void* dy_, int64_t ldd
             P o;
             if (act != ACT_NONE) {
                 const P z = *reinterpret_cast<const P*>(static_cast<const T*>(pre_) + m * N + n);
+                float zv[V], sl[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) zv[e] = (float)z.v[e];
+                act_slopes<V>(zv, sl, act);
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    const float g = (float)d.v[e] * act_slope((float)z.v[e], act);
+                    const float g = (float)d.v[e] * sl[e];
                     sum[e] += g;
                     o.v[e] = (T)g;
                 }
@@ -541,9 +652,9 @@ struct Plan { int tile; int splits; int64_t k_split; size_t part_bytes; };      
 Plan plan_product(int64_t M, int N, int64_t K, int dt, bool acol, bool bcol) {
     Plan p{0, 1, K, 0};
     if (!acol && !bcol && M <= 64) return p;
-    const int64_t ke = 128 / dtype_bytes(dt);
+    const int64_t ke = 128 / dtype_bytes(dt);                 // K step of the tiles
     auto tiles = [&](int64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
-    p.tile = (dt != DT_F32 && tiles(256) >= 200) ? 256 : tiles(128) >= 200 ? 128 : 64;
+    p.tile = tiles(256) >= 200 ? 256 : tiles(128) >= 200 ? 128 : 64;
     const int64_t steps = (K + ke - 1) / ke;
     p.k_split = steps * ke;
     if (p.tile == 64 && tiles(64) < 256) {
@@ -561,12 +672,11 @@ Plan plan_product(int64_t M, int N, int64_t K, int dt, bool acol, bool bcol) {
 }
 
 template <typename T, bool ACOL, bool BCOL, int EDGE>
-void launch_tile(const ProductArgs& a, bool dma, hipStream_t s) {
-    constexpr int WM = 2, WN = EDGE == 256 ? 4 : 2;
+void launch_tile(const ProductArgs& a, hipStream_t s) {
     const int n_tiles = a.tiles_m * a.tiles_n;
     const dim3 grid((unsigned)((n_tiles + 7) / 8 * 8), (unsigned)a.splits);
-    if (dma) hipLaunchKernelGGL((product_kernel<T, ACOL, BCOL, EDGE, EDGE, WM, WN, true>), grid, dim3(64 * WM * WN), 0, s, a);
-    else if constexpr (EDGE == 64) hipLaunchKernelGGL((product_kernel<T, ACOL, BCOL, EDGE, EDGE, WM, WN, false>), grid, dim3(64 * WM * WN), 0, s, a);
+    constexpr int WN = EDGE == 256 ? 4 : 2;
+    hipLaunchKernelGGL((product_kernel<T, ACOL, BCOL, EDGE, EDGE, 2, WN, 128, 2>), grid, dim3(128 * WN), 0, s, a);
 }
 
 template <typename T, int MT, int NT, int NWAVES>
@@ -584,6 +694,7 @@ hipError_t product(ProductArgs a, int dt, bool acol, bool bcol, void* part, hipS
     a.vec = a.N % V == 0 && a.ldy % V == 0 && on16(a.y) && on16(a.bias) && (!a.res || (on16(a.res) && a.ldr % V == 0)) && on16(a.pre);
     // operands by 16-byte pieces: rows start on 16 bytes and whole pieces make up the contiguous axis
     const bool pieces = on16(a.A) && on16(a.B) && a.lda % V == 0 && a.ldb % V == 0 && (acol ? a.M : a.K) % V == 0 && (bcol ? a.N : a.K) % V == 0;
+    const bool near = a.lda < (1 << 21) && a.ldb < (1 << 21);  // a tile's 256 rows span less than 2^31 bytes
     if (p.tile == 0) {
         with_dtype(dt, [&](auto t) {
             typedef decltype(t) T;
@@ -593,7 +704,8 @@ hipError_t product(ProductArgs a, int dt, bool acol, bool bcol, void* part, hipS
         });
         return hipGetLastError();
     }
-    if (!pieces && p.tile != 64) p.tile = 64;                  // operands that need element loads: the small tile, as many splits as planned (none)
+    const bool any = !pieces || !near;
+    if (any) p.tile = 64;
     a.splits = p.splits; a.k_split = p.k_split; a.part = static_cast<float*>(part);
     a.tiles_m = (int)((a.M + p.tile - 1) / p.tile); a.tiles_n = (a.N + p.tile - 1) / p.tile;
     if ((int64_t)a.tiles_m * a.tiles_n > 0x3FFFFFFF) return hipErrorInvalidValue;
@@ -601,9 +713,10 @@ hipError_t product(ProductArgs a, int dt, bool acol, bool bcol, void* part, hipS
         typedef decltype(t) T;
         auto by_tile = [&](auto ac, auto bc) {
             constexpr bool AC = decltype(ac)::value, BC = decltype(bc)::value;
-            if (p.tile == 256) { if constexpr (sizeof(T) == 2) launch_tile<T, AC, BC, 256>(a, pieces, s); }
-            else if (p.tile == 128) launch_tile<T, AC, BC, 128>(a, pieces, s);
-            else launch_tile<T, AC, BC, 64>(a, pieces, s);
+            if (any) hipLaunchKernelGGL((product_any_kernel<T, AC, BC>), dim3((unsigned)(a.tiles_m * a.tiles_n), (unsigned)a.splits), dim3(256), 0, s, a);
+            else if (p.tile == 256) launch_tile<T, AC, BC, 256>(a, s);
+            else if (p.tile == 128) launch_tile<T, AC, BC, 128>(a, s);
+            else launch_tile<T, AC, BC, 64>(a, s);
         };
         if (acol) by_tile(std::true_type{}, std::true_type{});
         else if (bcol) by_tile(std::false_type{}, std::true_type{});

@@ -2,13 +2,14 @@
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import Optional, Sequence
 
 import torch
 
 from . import _lib
-from ._lib import DTYPES, StepCoef, check, current_stream, f32c, on_device, ptr
+from ._lib import DTYPES, StepCoef, check, current_stream, device_of, f32c, on_data_device, ptr, stream_on
 
 
 def timestep_embedding(t: torch.Tensor, dim: int) -> torch.Tensor:
@@ -272,6 +273,7 @@ def rope_frequencies(rotary_dim: int, theta: float = 1e4, scaling: Optional[str]
     return inv.to(device), amplitude
 
 
+@on_data_device
 def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions, inv_freq: torch.Tensor, amplitude: float = 1.0, layout: str = "half",
          inverse: bool = False, inplace: bool = False):
     """Rotary positions of q (B, S, Hq, dh) and k (B, S, Hk, dh) -- or (N, H, dh) for packed tokens -- in one launch -> (q', k').
@@ -280,58 +282,57 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions, inv_freq: torch.
     fp64 and ``amplitude`` as ``rope_frequencies`` gives them: the first rd <= dh values of a head are rotated, the others copied.  ``layout``:
     "half" pairs (j, j + rd / 2), "interleaved" (2 j, 2 j + 1).  fp32, bf16 or fp16; any strides with adjacent values in a head (a slice of
     a fused q / k / v product, heads before tokens as a transposed view).  ``inverse`` applies the transpose -- the gradient.
-    ``inplace`` writes into q and k."""
-    if layout not in ("half", "interleaved"):
+    ``inplace`` writes into q and k, which must not overlap each other."""
+    if layout != "half" and layout != "interleaved":
         raise ValueError(f"rope: unknown layout {layout!r}")
-    dt = DTYPES.get(q.dtype)
-    if dt is None or (k is not None and k.dtype != q.dtype):
+    dtype, shape = q.dtype, q.shape
+    dt, axes = DTYPES.get(dtype), len(shape)
+    if dt is None or (k is not None and k.dtype != dtype):
         raise ValueError("rope: q and k are fp32, bf16 or fp16, both the same")
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("rope: inv_freq is a contiguous fp64 vector (rope_frequencies)")
-    if q.dim() not in (3, 4) or (k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1])):
+    if axes not in (3, 4) or (k is not None and (k.shape[:-2] != shape[:-2] or k.shape[-1] != shape[-1])):
         raise ValueError("rope: q (B, S, Hq, dh) and k (B, S, Hk, dh), or (N, Hq, dh) and (N, Hk, dh)")
-    dh, rd = q.shape[-1], 2 * inv_freq.numel()
-    if rd > dh or rd == 0 or q.shape[-2] == 0 or (k is not None and k.shape[-2] == 0):
+    hq, dh, rd = shape[-2], shape[-1], 2 * inv_freq.shape[0]
+    hk = 0 if k is None else k.shape[-2]
+    if rd > dh or rd == 0 or hq == 0 or (k is not None and hk == 0):
         raise ValueError(f"rope: {rd} rotated values of heads of {dh}, and at least one head")
-    if k is not None and inplace and k.numel() and k.data_ptr() == q.data_ptr():
-        raise ValueError("rope: q and k in place are the same tensor")
-    pos = positions if torch.is_tensor(positions) else None
-    with on_device("rope", q, k, pos, inv_freq) as stream:
-        if inplace:
-            for t in (q, k):
-                if t is not None and dh > 1 and t.stride(-1) != 1:
-                    raise ValueError("rope: in place needs adjacent values in a head")
-                if t is not None and any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
-                    raise ValueError("rope: in place needs a tensor without repeated elements")
-            qo, ko = q, k
-        else:
-            q = q if dh == 1 or q.stride(-1) == 1 else q.contiguous()
-            qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            ko = None
-            if k is not None:
-                k = k if dh == 1 or k.stride(-1) == 1 else k.contiguous()
-                ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        lead = q.shape[:-2]
-        B, S = lead if len(lead) == 2 else (1, lead[0])
-        if B * S == 0:
-            return qo, ko
-        pb = ps = 0
-        if pos is not None:
-            if pos.dtype != torch.int64:
-                raise ValueError("rope: positions are int64")
-            pos = pos.expand(lead)
-            ps, pb = pos.stride(-1), pos.stride(0) if len(lead) == 2 else 0
-        st = []
-        for t in (q, qo, k, ko):
-            if t is None:
-                st += (0, 0, 0)
-            else:
-                ts = t.stride()
-                st += ts[:3] if len(lead) == 2 else (0, ts[0], ts[1])
-        check(_lib.load().adx_op_rope(q.data_ptr(), qo.data_ptr(), q.shape[-2], None if k is None else k.data_ptr(), None if ko is None else ko.data_ptr(),
-                                      0 if k is None else k.shape[-2], _Strides(*st), None if pos is None else pos.data_ptr(), pb, ps,
-                                      0 if pos is not None else int(positions), inv_freq.data_ptr(), float(amplitude), B, S, dh, rd,
-                                      int(layout == "interleaved"), int(inverse), dt, stream), "rope")
+    pos = positions if isinstance(positions, torch.Tensor) else None
+    if pos is not None and pos.dtype != torch.int64:
+        raise ValueError("rope: positions are int64")
+    if inplace:
+        for t in (q, k):
+            if t is not None and dh > 1 and t.stride(-1) != 1:
+                raise ValueError("rope: in place needs adjacent values in a head")
+            if t is not None and any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+                raise ValueError("rope: in place needs a tensor without repeated elements")
+        if k is not None and k.numel() and k.data_ptr() == q.data_ptr():
+            raise ValueError("rope: q and k in place are the same memory")
+    stream = stream_on(device_of("rope", q, k, pos, inv_freq))
+    if inplace:
+        qo, ko = q, k
+    else:
+        if dh > 1 and q.stride(-1) != 1:
+            q = q.contiguous()
+        if k is not None and dh > 1 and k.stride(-1) != 1:
+            k = k.contiguous()
+        qo, ko = q.new_empty(shape), None if k is None else k.new_empty(k.shape)
+    S = shape[-3]
+    B = shape[0] if axes == 4 else 1
+    if B * S == 0:
+        return qo, ko
+    pb = ps = 0
+    if pos is not None:
+        if pos.shape != shape[:-2]:
+            pos = pos.expand(shape[:-2])
+        ps = pos.stride(-1)
+        pb = pos.stride(0) if axes == 4 else 0
+    outer = (0,) if axes == 3 else ()
+    st = outer + q.stride()[:-1] + outer + qo.stride()[:-1]
+    st += (0,) * 6 if k is None else outer + k.stride()[:-1] + outer + ko.stride()[:-1]
+    check(_lib.load().adx_op_rope(q.data_ptr(), qo.data_ptr(), hq, None if k is None else k.data_ptr(), None if k is None else ko.data_ptr(), hk,
+                                  _Strides(*st), None if pos is None else pos.data_ptr(), pb, ps, 0 if pos is not None else int(positions),
+                                  inv_freq.data_ptr(), amplitude, B, S, dh, rd, layout == "interleaved", inverse, dt, stream), "rope")
     return qo, ko
 
 
@@ -339,71 +340,87 @@ def _rows(t: torch.Tensor):
     """(tensor, row stride) of t viewed as rows of its last axis, copied only where its strides do not allow the view."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    rows, width = t.shape
+    if width > 1 and t.stride(1) != 1:
         t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+    return t, (t.stride(0) if rows > 1 else width)
 
 
+@functools.lru_cache(maxsize=4096)
+def _linear_residual_bytes(M: int, N: int, K: int, dt: int, act: int = -1) -> int:
+    lib = _lib.load()
+    return int(lib.adx_linear_residual_ws_bytes(M, N, K, dt) if act < 0 else lib.adx_linear_residual_bwd_ws_bytes(M, N, K, act, dt))
+
+
+@on_data_device
 def linear_residual(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
                     act: int = _lib.ACT_NONE, keep_pre: bool = False):
     """``act(x w^T + bias) + residual`` in the tensors' own type (fp32, bf16 or fp16, all the same; fp32 sums, one rounding): x (..., K),
     w (N, K), bias (N,), residual (..., N).  ``act``: ACT_NONE .. ACT_TANH.  ``keep_pre`` also returns the value before the activation, which
     ``linear_residual_bwd`` needs.  Rows of x, w and residual may be strided (adjacent values in a row)."""
-    dt = DTYPES.get(x.dtype)
-    if dt is None or any(t is not None and t.dtype != x.dtype for t in (w, bias, residual)):
+    dtype = x.dtype
+    dt = DTYPES.get(dtype)
+    if dt is None or w.dtype != dtype or (bias is not None and bias.dtype != dtype) or (residual is not None and residual.dtype != dtype):
         raise ValueError("linear_residual: x, w, bias and residual are fp32, bf16 or fp16, all the same")
-    if x.dim() < 1 or w.dim() != 2 or w.shape[1] != x.shape[-1] or w.shape[0] == 0 or w.shape[1] == 0:
+    if w.dim() != 2 or x.dim() < 1:
         raise ValueError("linear_residual: x (..., K) and w (N, K)")
     N, K = w.shape
-    out_shape = x.shape[:-1] + (N,)
+    if x.shape[-1] != K or N == 0 or K == 0:
+        raise ValueError("linear_residual: x (..., K) and w (N, K)")
+    out_shape = (*x.shape[:-1], N)
     if (bias is not None and bias.shape != (N,)) or (residual is not None and residual.shape != out_shape):
         raise ValueError("linear_residual: bias (N,) and residual of the output's shape")
-    lib = _lib.load()
-    with on_device("linear_residual", x, w, bias, residual) as stream:
-        y = torch.empty(out_shape, dtype=x.dtype, device=x.device)
-        pre = torch.empty(out_shape, dtype=x.dtype, device=x.device) if keep_pre else None
-        x2, ldx = _rows(x)
-        M = x2.shape[0]
-        if M:
-            w2, ldw = _rows(w)
-            b = None if bias is None else bias.contiguous()
-            r2, ldr = (None, 0) if residual is None else _rows(residual)
-            need = lib.adx_linear_residual_ws_bytes(M, N, K, dt)
-            ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-            check(lib.adx_op_linear_residual(x2.data_ptr(), ldx, w2.data_ptr(), ldw, None if b is None else b.data_ptr(),
-                                             None if r2 is None else r2.data_ptr(), ldr, None if pre is None else pre.data_ptr(), y.data_ptr(), N, M, N, K,
-                                             act, dt, None if ws is None else ws.data_ptr(), need, stream), "linear_residual")
+    stream = stream_on(device_of("linear_residual", x, w, bias, residual))
+    y = x.new_empty(out_shape)
+    pre = x.new_empty(out_shape) if keep_pre else None
+    x2, ldx = _rows(x)
+    M = x2.shape[0]
+    if M:
+        w2, ldw = _rows(w)
+        b = None if bias is None else bias.contiguous()
+        r2, ldr = (None, 0) if residual is None else _rows(residual)
+        need = _linear_residual_bytes(M, N, K, dt)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        check(_lib.load().adx_op_linear_residual(x2.data_ptr(), ldx, w2.data_ptr(), ldw, None if b is None else b.data_ptr(),
+                                                 None if r2 is None else r2.data_ptr(), ldr, None if pre is None else pre.data_ptr(), y.data_ptr(), N,
+                                                 M, N, K, act, dt, None if ws is None else ws.data_ptr(), need, stream), "linear_residual")
     return (y, pre) if keep_pre else y
 
 
+@on_data_device
 def linear_residual_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pre: Optional[torch.Tensor] = None, act: int = _lib.ACT_NONE,
                         need_dx: bool = True, need_dw: bool = True, need_db: bool = True):
     """(dx, dw, db) of ``linear_residual`` from the gradient of its output, its operands and (unless act is ACT_NONE) the value before
     the activation; None for those not asked for.  The gradient of the residual is dy."""
-    dt = DTYPES.get(dy.dtype)
-    if dt is None or any(t is not None and t.dtype != dy.dtype for t in (x, w, pre)):
+    dtype = dy.dtype
+    dt = DTYPES.get(dtype)
+    if dt is None or x.dtype != dtype or w.dtype != dtype or (pre is not None and pre.dtype != dtype):
         raise ValueError("linear_residual_bwd: dy, x, w and pre are fp32, bf16 or fp16, all the same")
+    if w.dim() != 2 or x.dim() < 1:
+        raise ValueError("linear_residual_bwd: x (..., K), w (N, K), dy and pre (..., N)")
     N, K = w.shape
-    if x.shape[-1] != K or dy.shape != x.shape[:-1] + (N,) or (pre is not None and pre.shape != dy.shape):
+    if x.shape[-1] != K or dy.shape != (*x.shape[:-1], N) or (pre is not None and pre.shape != dy.shape):
         raise ValueError("linear_residual_bwd: x (..., K), w (N, K), dy and pre (..., N)")
     if act != _lib.ACT_NONE and pre is None:
         raise ValueError("linear_residual_bwd: the activation's gradient needs pre (linear_residual with keep_pre)")
-    lib = _lib.load()
-    with on_device("linear_residual_bwd", dy, x, w, pre) as stream:
-        g, ldd = _rows(dy)
-        M = g.shape[0]
-        make = torch.empty if M else torch.zeros
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_dx else None
-        dw = make(N, K, dtype=w.dtype, device=w.device) if need_dw else None
-        db = make(N, dtype=w.dtype, device=w.device) if need_db else None
-        if M and (need_dx or need_dw or need_db):
-            x2, ldx = _rows(x)
-            w2, ldw = _rows(w)
-            z = None if pre is None else pre.contiguous()
-            need = lib.adx_linear_residual_bwd_ws_bytes(M, N, K, act, dt)
-            ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-            check(lib.adx_op_linear_residual_bwd(g.data_ptr(), ldd, x2.data_ptr(), ldx, w2.data_ptr(), ldw, None if z is None else z.data_ptr(),
-                                                 None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
-                                                 None if db is None else db.data_ptr(), M, N, K, act, dt, ws.data_ptr(), need, stream),
-                  "linear_residual_bwd")
+    stream = stream_on(device_of("linear_residual_bwd", dy, x, w, pre))
+    g, ldd = _rows(dy)
+    M = g.shape[0]
+    dx = x.new_empty(x.shape) if need_dx else None
+    dw = w.new_empty((N, K)) if need_dw else None
+    db = w.new_empty((N,)) if need_db else None
+    if M == 0:                                           # sums over no rows
+        for t in (dw, db):
+            if t is not None:
+                t.zero_()
+    elif need_dx or need_dw or need_db:
+        x2, ldx = _rows(x)
+        w2, ldw = _rows(w)
+        z = None if pre is None else pre.contiguous()
+        need = _linear_residual_bytes(M, N, K, dt, act)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        check(_lib.load().adx_op_linear_residual_bwd(g.data_ptr(), ldd, x2.data_ptr(), ldx, w2.data_ptr(), ldw, None if z is None else z.data_ptr(),
+                                                     None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
+                                                     None if db is None else db.data_ptr(), M, N, K, act, dt, ws.data_ptr(), need, stream),
+              "linear_residual_bwd")
     return dx, dw, db

@@ -24,6 +24,7 @@ arithmetic.  Every arithmetic step is a libadx kernel (``adx_op_rmsnorm``, ``adx
 """
 from __future__ import annotations
 
+import functools
 from types import SimpleNamespace
 from typing import Dict, List, Optional
 
@@ -31,7 +32,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib, ops
-from ._lib import DTYPES, check, current_stream, f32c, on_device, ptr
+from ._lib import DTYPES, check, current_stream, device_of, f32c, on_data_device, ptr, stream_on
 from .raster_encoder import NuplanRasterizeEncoder, _add, _tanh
 from .refiner import _Lin
 from .trajectory_decoder import TrajectoryDecoder
@@ -88,43 +89,52 @@ def prepare_expert_weights(w1: List[torch.Tensor], w3: List[torch.Tensor], w2: L
             ops.prepare_weight(wd.reshape(-1, wd.shape[-1]), precision).reshape(-1))
 
 
+_FEW_WEIGHTS = {"fp32": (torch.float32,), "bf16": (torch.bfloat16, torch.int16), "bf16x3": (torch.int16, torch.bfloat16), "f16": (torch.float16, torch.int16)}
+
+
+@functools.lru_cache(maxsize=4096)
+def _moe_few_bytes(T: int, d: int, inter: int, n_experts: int, top_k: int, dt: int, prec: int) -> int:
+    return int(_lib.load().adx_moe_few_workspace_bytes(T, d, inter, n_experts, top_k, dt, prec))
+
+
+@on_data_device
 def moe_few(x: torch.Tensor, res: Optional[torch.Tensor], router_w: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, inter: int, n_experts: int,
             top_k: int, precision: str = "fp32", workspace: Optional[torch.Tensor] = None, return_routing: bool = False):
     """``moe_block`` for at most 64 tokens in two kernels.  x, res (T, d) fp32 with weights of any ``precision`` ("fp32" | "bf16" | "bf16x3" |
     "f16"), or bf16 with "bf16", or fp16 with "f16" weights; returns x's type.  w13 / w2: as ``prepare_expert_weights`` returns them, or the
     plain (E, 2 inter, d) / (E, d, inter) tensors of that type.  router_w (E, d) fp32."""
-    dt, prec = DTYPES.get(x.dtype), _lib.PRECISIONS[precision]
-    if dt is None or x.dim() != 2 or (res is not None and (res.dtype != x.dtype or res.shape != x.shape)):
+    dtype = x.dtype
+    dt, prec, kinds = DTYPES.get(dtype), _lib.PRECISIONS[precision], _FEW_WEIGHTS.get(precision)
+    if dt is None or x.dim() != 2 or (res is not None and (res.dtype != dtype or res.shape != x.shape)):
         raise ValueError("moe_few: x (T, d) and res of its shape, fp32, bf16 or fp16")
+    if kinds is None:
+        raise ValueError(f"moe_few: no form of the weights under precision {precision!r}")
     T, d = x.shape
-    planes = 2 if precision == "bf16x3" else 1
-    wide = 4 if precision == "fp32" else 2
     if router_w.dtype != torch.float32 or router_w.shape != (n_experts, d):
         raise ValueError("moe_few: router_w (E, d) fp32")
-    for w, n in ((w13, 2 * inter * d), (w2, inter * d)):
-        if w.numel() != planes * n_experts * n or w.element_size() != wide or not w.is_contiguous():
-            raise ValueError("moe_few: w13 and w2 hold (E, 2 inter, d) and (E, d, inter) contiguous values in the form of their precision")
-        if w.dtype not in ((torch.float32,) if wide == 4 else (torch.int16, torch.float16 if precision == "f16" else torch.bfloat16)):
-            raise ValueError(f"moe_few: {w.dtype} weights under precision {precision!r}")
-    lib = _lib.load()
-    with on_device("moe_few", x, res, router_w, w13, w2, workspace) as stream:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        if T == 0:
-            none = torch.empty(0, top_k, device=x.device)
-            return (y, none.int(), none) if return_routing else y
-        x, router_w = x.contiguous(), router_w.contiguous()
-        res = None if res is None else res.contiguous()
-        need = lib.adx_moe_few_workspace_bytes(T, d, inter, n_experts, top_k, dt, prec)
-        if workspace is None or workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
-            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-        check(lib.adx_op_moe_few(x.data_ptr(), None if res is None else res.data_ptr(), router_w.data_ptr(), w13.data_ptr(), w2.data_ptr(), T, d, inter,
-                                 n_experts, top_k, dt, prec, workspace.data_ptr(), workspace.numel() * workspace.element_size(), y.data_ptr(), stream),
-              "moe_few")
-        if not return_routing:
-            return y
-        n = T * top_k
-        flat, off = workspace.reshape(-1).view(torch.uint8), (n * 4 + 255) // 256 * 256
-        return y, flat[:n * 4].view(torch.int32).reshape(T, top_k).clone(), flat[off:off + n * 4].view(torch.float32).reshape(T, top_k).clone()
+    n = n_experts * inter * d * (2 if precision == "bf16x3" else 1)
+    if w13.numel() != 2 * n or w2.numel() != n or not (w13.is_contiguous() and w2.is_contiguous()):
+        raise ValueError("moe_few: w13 and w2 hold (E, 2 inter, d) and (E, d, inter) contiguous values in the form of their precision")
+    if w13.dtype not in kinds or w2.dtype not in kinds:
+        raise ValueError(f"moe_few: {w13.dtype} and {w2.dtype} weights under precision {precision!r}")
+    stream = stream_on(device_of("moe_few", x, res, router_w, w13, w2, workspace))
+    y = x.new_empty((T, d))
+    if T == 0:
+        none = x.new_empty((0, top_k), dtype=torch.float32)
+        return (y, none.int(), none) if return_routing else y
+    x, router_w = x.contiguous(), router_w.contiguous()
+    res = None if res is None else res.contiguous()
+    need = _moe_few_bytes(T, d, inter, n_experts, top_k, dt, prec)
+    if workspace is None or workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
+        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    check(_lib.load().adx_op_moe_few(x.data_ptr(), None if res is None else res.data_ptr(), router_w.data_ptr(), w13.data_ptr(), w2.data_ptr(), T, d, inter,
+                                     n_experts, top_k, dt, prec, workspace.data_ptr(), workspace.numel() * workspace.element_size(), y.data_ptr(), stream),
+          "moe_few")
+    if not return_routing:
+        return y
+    n = T * top_k
+    flat, off = workspace.reshape(-1).view(torch.uint8), (n * 4 + 255) // 256 * 256
+    return y, flat[:n * 4].view(torch.int32).reshape(T, top_k).clone(), flat[off:off + n * 4].view(torch.float32).reshape(T, top_k).clone()
 
 
 class _RMS(nn.Module):

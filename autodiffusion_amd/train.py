@@ -822,26 +822,32 @@ def denoise_dit_with_grad(module: torch.nn.Module, x, t, state) -> torch.Tensor:
 
 
 # ------------------------------------------------------------------------------------------------ decoder-layer operators (fp32 / bf16 / fp16)
+def _first_order(what: str) -> None:
+    if torch.is_grad_enabled():                          # only while a graph of the backward pass itself is recorded
+        raise RuntimeError(f"{what}: gradients of gradients are not built")
+
+
 class _Rope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, amplitude, layout):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions if torch.is_tensor(positions) else None, inv_freq)
-        ctx.first, ctx.amplitude, ctx.layout = (None if torch.is_tensor(positions) else positions), amplitude, layout
+        at_tensor = isinstance(positions, torch.Tensor)
+        ctx.save_for_backward(positions if at_tensor else None, inv_freq)
+        ctx.first, ctx.amplitude, ctx.layout = None if at_tensor else positions, amplitude, layout
         qo, ko = ops.rope(q, k, positions, inv_freq, amplitude, layout)
         return qo if k is None else (qo, ko)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk=None):
+        _first_order("rope")
         positions, inv_freq = ctx.saved_tensors
         at = ctx.first if positions is None else positions
         if dq is None and dk is None:
             return None, None, None, None, None, None
         if dq is None:                                   # only the keys' outputs were used
-            dk, _ = ops.rope(dk, None, at, inv_freq, ctx.amplitude, ctx.layout, inverse=True)
+            dk, _ = ops.rope(dk, None, at, inv_freq, ctx.amplitude, ctx.layout, True)
         else:
-            dq, dk = ops.rope(dq, dk, at, inv_freq, ctx.amplitude, ctx.layout, inverse=True)
+            dq, dk = ops.rope(dq, dk, at, inv_freq, ctx.amplitude, ctx.layout, True)
         return dq, dk, None, None, None, None
 
 
@@ -855,24 +861,27 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions, inv_freq: torch.
 class _LinearResidual(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, act_code):
-        need = any(ctx.needs_input_grad[:3])
+        need = ctx.needs_input_grad
+        grad = need[0] or need[1] or need[2]
         pre = None
-        if need and act_code != _lib.ACT_NONE:
-            y, pre = ops.linear_residual(x, w, bias, residual, act_code, keep_pre=True)
+        if grad and act_code != _lib.ACT_NONE:
+            y, pre = ops.linear_residual(x, w, bias, residual, act_code, True)
         else:
             y = ops.linear_residual(x, w, bias, residual, act_code)
         ctx.act_code = act_code
-        ctx.save_for_backward(x if need else None, w if need else None, pre)
+        if grad:
+            ctx.save_for_backward(x, w, pre)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w, pre = ctx.saved_tensors
+        _first_order("linear_residual")
+        need = ctx.needs_input_grad
         dx = dw = db = None
-        if x is not None:
-            dx, dw, db = ops.linear_residual_bwd(dy, x, w, pre, ctx.act_code, *ctx.needs_input_grad[:3])
-        return dx, dw, db, dy if ctx.needs_input_grad[3] else None, None
+        if need[0] or need[1] or need[2]:
+            x, w, pre = ctx.saved_tensors
+            dx, dw, db = ops.linear_residual_bwd(dy, x, w, pre, ctx.act_code, need[0], need[1], need[2])
+        return dx, dw, db, dy if need[3] else None, None
 
 
 def linear_residual(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
