@@ -19,19 +19,17 @@ OBJ = os.path.join(HERE, "csrc", "build")
 SOURCES = ["kernels.hip", "gemm.hip", "attn_mfma.hip", "modes.hip", "metrics.hip", "extras.hip", "fused_a.hip", "tail_a.hip", "tail_mfma.hip", "engine_base.hip", "engine_a.hip", "engine_dit.hip", "noalloc.hip", "backward.hip", "raster.hip", "moe.hip", "rope.hip", "product.hip", "moe_few.hip"]
 HEADERS = ["adx_ops.h", "fastmath.h", "typed.h", "engine.h", os.path.join("..", "..", "include", "adx.h")]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wno-unused-function",
-         # no packed fp32 arithmetic (v_pk_add / mul / fma_f32): some of its forms have given wrong results on this hardware
-         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Rpass-analysis=kernel-resource-usage"]
-# scalar fp32 code is longer: the epilogues of the product kernels would pass the limit up to which `#pragma unroll` is obeyed
-EXTRA = {"gemm.hip": ["-mllvm", "-pragma-unroll-threshold=262144"]}
+         "-Rpass-analysis=kernel-resource-usage"]
+# Sources compiled without packed fp32 arithmetic (v_pk_add / mul / fma_f32).
+NO_PACKED_FP32 = {"rope.hip", "product.hip", "moe_few.hip"}
 # Kernels that must not touch scratch memory: their accumulators or row state live in registers by design, and a loop that stops
 # unrolling (the accumulators are indexed by its counter) silently moves them to scratch -- same results, a quarter slower.
 NO_SCRATCH = re.compile(r"linear_\w*kernel|mlp256_kernel|enc_rows_kernel|attn_g_kernel|tail_mfma_kernel|attn_bf_kernel|attn_mfma\w*kernel|"
                         r"layernorm_\w*kernel|product_\w*kernel|few_\w*kernel")
 
 
-# known and accepted: the 4-waves-per-SIMD instances of the row kernel (a tuning alternative, not the default) and two instances of the
-# fused MLP on split operands spill a few registers
-SCRATCH_OK = re.compile(r"enc_rows_kernelILi\dELi4E|mlp256_kernelILb1E")
+# known and accepted: the 4-waves-per-SIMD instances of the row kernel (a tuning alternative, not the default) spill a few registers
+SCRATCH_OK = re.compile(r"enc_rows_kernelILi\dELi4E")
 
 
 def _scratch_users(remarks: str):
@@ -71,7 +69,8 @@ def build(force: bool = False, verbose: bool = True, measure: bool = False) -> s
         o = os.path.join(obj_dir, src.replace(".hip", ".o"))
         objs.append(o)
         if force or _stale(o, [s] + hdrs):
-            jobs.append([hipcc, *flags, *EXTRA.get(src, []), "-c", s, "-o", o])
+            extra = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] if src in NO_PACKED_FP32 else []
+            jobs.append([hipcc, *flags, *extra, "-c", s, "-o", o])
 
     def run(cmd):
         if verbose:
@@ -87,7 +86,7 @@ def build(force: bool = False, verbose: bool = True, measure: bool = False) -> s
         if verbose and other.strip():
             print(other, file=sys.stderr)
 
-    with ThreadPoolExecutor(max_workers=6) as ex:
+    with ThreadPoolExecutor(max_workers=4) as ex:
         list(ex.map(run, jobs))
     if jobs or force or _stale(out, objs):
         run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out, *objs])
