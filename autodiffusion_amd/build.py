@@ -20,7 +20,8 @@ SOURCES = ["kernels.hip", "gemm.hip", "attn_mfma.hip", "modes.hip", "metrics.hip
 HEADERS = ["adx_ops.h", "fastmath.h", "typed.h", "engine.h", os.path.join("..", "..", "include", "adx.h")]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wno-unused-function",
          "-Rpass-analysis=kernel-resource-usage"]
-# Sources compiled without packed fp32 arithmetic (v_pk_add / mul / fma_f32).
+# Sources compiled without packed fp32 arithmetic (v_pk_add / mul / fma_f32): some of its forms have given wrong results on this hardware.
+# The others keep it: their results are pinned with it (without it the refiner's fp16 engine leaves its ADE bound: the contractions change).
 NO_PACKED_FP32 = {"rope.hip", "product.hip", "moe_few.hip"}
 # Kernels that must not touch scratch memory: their accumulators or row state live in registers by design, and a loop that stops
 # unrolling (the accumulators are indexed by its counter) silently moves them to scratch -- same results, a quarter slower.

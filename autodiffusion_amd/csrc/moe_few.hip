@@ -29,15 +29,20 @@ constexpr int FEW_MAX_T = 64, FEW_MAX_K = 8, FEW_MAX_E = 64;
 constexpr int WAVES = 8;                                  // of a workgroup of either product
 enum : int { P_F32 = 0, P_BF16 = 1, P_BF16X3 = 2, P_F16 = 4 };         // the ADX_PREC_* codes
 
+// Sizes of the launches, each the best of a sweep on 1 .. 64 tokens of widths 256 .. 1536: `up` at most so many workgroups; `down` at
+// least so many, and enough that none reads more than so many KB of weights
+constexpr int UP_BLOCKS = 768, DOWN_BLOCKS = 256, DOWN_KB = 192;
+
 struct FewArgs {
     const void* x; const void* res; const float* router;
     const void* w13; const void* w2;
     int T, d, inter, E, top_k;
     int* idx; float* wts;                                 // [T][top_k]
-    int* table; int active;                               // `up` -> `down`: [active] rows of {expert or -1, count, entries (token * top_k + slot)[T]}
+    int* table;                                           // `up` -> `down`: how many experts were chosen, and a row {expert, count, entries (token * top_k + slot)[T]} each
     void* h; int64_t h_plane;                             // hidden rows [part][T top_k][inter]; elements of one part
-    float* part; int* arrived;                            // shares > 1: [shares][T][d], [d / 16]
-    int shares, k_splits;
+    float* part;                                          // [k_splits][T top_k][d]
+    int* arrived; int arrivals;                           // workgroups of `down` that are done, a column group
+    int wk, k_splits;
     void* y;
 };
 
@@ -65,6 +70,17 @@ __device__ __forceinline__ float wave_max(float v) {
     v = fmaxf(v, dpp<HALF_MIRROR>(v));
     v = fmaxf(v, dpp<MIRROR>(v));
     return xor32_max(xor16_max(v));
+}
+
+__device__ __forceinline__ unsigned wave_or(unsigned v) {
+    v |= __float_as_uint(dpp<QUAD_SWAP1>(__uint_as_float(v)));
+    v |= __float_as_uint(dpp<QUAD_SWAP2>(__uint_as_float(v)));
+    v |= __float_as_uint(dpp<HALF_MIRROR>(__uint_as_float(v)));
+    v |= __float_as_uint(dpp<MIRROR>(__uint_as_float(v)));
+    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = r[0] | r[1];
+    r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return r[0] | r[1];
 }
 
 // ------------------------------------------------------------------------------------------------------------- operand fragments
@@ -114,11 +130,10 @@ template <int P> struct Weight {
     static constexpr int CE = P == P_F32 ? 4 : 8, SZ = P == P_F32 ? 4 : 2;
     static constexpr int RAW = P == P_BF16X3 ? 2 : 1, PARTS = P == P_BF16X3 || P == P_F16 ? 2 : 1;
     uint4 raw[RAW];
-    // `at`: element index of the first value; `low`: elements between the high and the low plane
-    __device__ __forceinline__ void load(const void* w, int64_t at, int64_t low) {
-        const unsigned char* p = static_cast<const unsigned char*>(w) + at * SZ;
-        raw[0] = *reinterpret_cast<const uint4*>(p);
-        if constexpr (RAW == 2) raw[1] = *reinterpret_cast<const uint4*>(p + low * SZ);
+    // `base`: the same for the whole wave; `at`: byte offset of the lane's first value; `low`: bytes between the high and the low plane
+    __device__ __forceinline__ void load(const unsigned char* base, unsigned at, int64_t low) {
+        raw[0] = *reinterpret_cast<const uint4*>(base + at);
+        if constexpr (RAW == 2) raw[1] = *reinterpret_cast<const uint4*>(base + low + at);
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -150,41 +165,62 @@ __device__ __forceinline__ f32x4_t mfma_parts(const uint4 (&w)[PW], const uint4 
 }
 
 // ------------------------------------------------------------------------------------------------------------- routing
-// The routing of tokens t0 .. t0 + n - 1 by a whole workgroup: every wave takes its part of the summed axis of one token and eight
-// experts, so that the loads of a logit are one round trip; then the choice, one token a wave.  `part`: n ceil(E / 8) * 64 floats of LDS.
-constexpr int ROUTE_GROUPS = 8;                           // tokens times groups of eight experts a call may hold in LDS
-template <typename A>
+// Sums of eight values a lane over the wave: lanes 0 .. 3 return value 4 (lane & 1) + 2 (lane >> 1) + i in r[i].  The first two steps
+// halve the values instead of keeping eight sums a lane.
+constexpr int ROTATE4 = 0x124, ROTATE8 = 0x128;            // rotations within 16 lanes
+__device__ __forceinline__ void wave_sum8(const float (&s)[8], int lane, float (&r)[2]) {
+    float p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = ((lane & 1) ? s[i + 4] : s[i]) + dpp<QUAD_SWAP1>((lane & 1) ? s[i] : s[i + 4]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float v = ((lane & 2) ? p[i + 2] : p[i]) + dpp<QUAD_SWAP2>((lane & 2) ? p[i] : p[i + 2]);
+        v += dpp<ROTATE4>(v);
+        v += dpp<ROTATE8>(v);
+        r[i] = xor32_add(xor16_add(v));
+    }
+}
+
+// The routing of tokens t0 .. t0 + n - 1 by a whole workgroup.  The waves spread over groups of eight experts and parts of the summed
+// axis; a wave reads its piece of the router once for all tokens.  Then the choice, one token a wave.  `part`: n ROUTE_WAVE floats of LDS.
+constexpr int ROUTE_TOKENS = 4, ROUTE_WAVE = WAVES * 8;           // tokens of one round
+template <typename A, int N>
 __device__ __forceinline__ void route(const FewArgs& a, int t0, int n, float* part, int* idx, float* wts) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int groups = (a.E + 7) / 8;
-    for (int p = 0; p < n * groups; ++p) {
-        const int t = p / groups, e0 = (p - t * groups) * 8;
-        const A* x = static_cast<const A*>(a.x) + (int64_t)(t0 + t) * a.d;
-        float s[8];
+    const int groups = (a.E + 7) / 8, parts = WAVES / groups, e0 = wave / parts * 8;        // WAVES >= 8 >= groups; waves beyond groups * parts rest
+    if (wave < groups * parts) {
+        float s[N][8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) s[q] = 0.f;
-        for (int i = threadIdx.x * 4; i < a.d; i += 256 * WAVES) {      // d is a multiple of 32
-            const Pack<A, 4> xv = *reinterpret_cast<const Pack<A, 4>*>(x + i);
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int q = 0; q < 8; ++q) s[t][q] = 0.f;
+        for (int i = (wave % parts * 64 + lane) * 4; i < a.d; i += 256 * parts) {          // d is a multiple of 32
             float4 wv[8];
+            Pack<A, 4> xv[N];
 #pragma unroll
             for (int q = 0; q < 8; ++q) wv[q] = *reinterpret_cast<const float4*>(a.router + (int64_t)min(e0 + q, a.E - 1) * a.d + i);
 #pragma unroll
-            for (int q = 0; q < 8; ++q) s[q] += (float)xv.v[0] * wv[q].x + (float)xv.v[1] * wv[q].y + (float)xv.v[2] * wv[q].z + (float)xv.v[3] * wv[q].w;
+            for (int t = 0; t < N; ++t) xv[t] = *reinterpret_cast<const Pack<A, 4>*>(static_cast<const A*>(a.x) + (int64_t)(t0 + min(t, n - 1)) * a.d + i);
+#pragma unroll
+            for (int t = 0; t < N; ++t)
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    s[t][q] += (float)xv[t].v[0] * wv[q].x + (float)xv[t].v[1] * wv[q].y + (float)xv[t].v[2] * wv[q].z + (float)xv[t].v[3] * wv[q].w;
         }
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            s[q] = wave_sum(s[q]);
-            if (lane == 0) part[(p * WAVES + wave) * 8 + q] = s[q];
+        for (int t = 0; t < N; ++t) {
+            float r[2];
+            wave_sum8(s[t], lane, r);
+            if (lane < 4 && t < n) *reinterpret_cast<float2*>(part + t * ROUTE_WAVE + wave * 8 + 4 * (lane & 1) + 2 * (lane >> 1)) = make_float2(r[0], r[1]);
         }
     }
     __syncthreads();
     for (int t = wave; t < n; t += WAVES) {
         float mine = -INFINITY;
         if (lane < a.E) {
-            const float* l = part + (t * groups + (lane >> 3)) * WAVES * 8 + (lane & 7);
+            const float* l = part + t * ROUTE_WAVE + (lane >> 3) * parts * 8 + (lane & 7);
             mine = 0.f;
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) mine += l[w * 8];
+            for (int w = 0; w < parts; ++w) mine += l[w * 8];
         }
         const float mx = wave_max(mine);
         const float ex = lane < a.E ? expf(mine - mx) : 0.f;
@@ -210,154 +246,170 @@ __device__ __forceinline__ void route(const FewArgs& a, int t0, int n, float* pa
 
 template <typename A>
 __global__ __launch_bounds__(64 * WAVES) void few_route_kernel(const FewArgs a) {
-    __shared__ float part[ROUTE_GROUPS * WAVES * 8];
+    __shared__ __attribute__((aligned(16))) float part[ROUTE_WAVE];
     const int t = blockIdx.x;
-    route<A>(a, t, 1, part, a.idx + t * a.top_k, a.wts + t * a.top_k);
+    route<A, 1>(a, t, 1, part, a.idx + t * a.top_k, a.wts + t * a.top_k);
 }
 
-// The `rank`-th expert (by index) that any token chose, -1 if there are fewer; its entries (token * top_k + slot) in token order
-struct Chosen {
-    int entry[FEW_MAX_T];
-    unsigned used[2];
-    int count;
-};
-__device__ __forceinline__ int chosen_expert(const int* idx, int n, int rank, unsigned* used) {
-    if (threadIdx.x < 2) used[threadIdx.x] = 0u;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += 64 * WAVES) atomicOr(&used[idx[i] >> 5], 1u << (idx[i] & 31));       // LDS; the result does not depend on the order
-    __syncthreads();
-    unsigned long long m = (unsigned long long)used[1] << 32 | used[0];
-    for (int i = 0; i < rank && m; ++i) m &= m - 1;
-    return m ? __ffsll((long long)m) - 1 : -1;
-}
-// the entries of expert e (a token chooses an expert once: at most T); executed by the whole workgroup
-__device__ __forceinline__ void entries_of(const int* idx, int n, int e, Chosen& c) {
-    __syncthreads();
-    if (threadIdx.x < 64) {
-        const int lane = threadIdx.x;
-        int base = 0;
-        for (int i0 = 0; i0 < n; i0 += 64) {
-            const bool hit = i0 + lane < n && idx[i0 + lane] == e;
-            const unsigned long long m = __ballot(hit);
-            if (hit) c.entry[base + __popcll(m & ((1ull << lane) - 1ull))] = i0 + lane;
-            base += __popcll(m);
-        }
-        if (lane == 0) c.count = base;
+// The `rank`-th expert (by index) that any token chose, -1 if there are fewer; `chosen`: how many there are.  Every wave finds it by itself.
+__device__ __forceinline__ int chosen_expert(const int* idx, int n, int rank, int lane, int* chosen) {
+    unsigned lo = 0, hi = 0;
+    for (int i = lane; i < n; i += 64) {
+        const int e = idx[i];
+        if (e < 32) lo |= 1u << e; else hi |= 1u << (e - 32);
     }
-    __syncthreads();
+    unsigned long long used = (unsigned long long)wave_or(hi) << 32 | wave_or(lo);
+    *chosen = __popcll(used);
+    for (int i = 0; i < rank && used; ++i) used &= used - 1;
+    return used ? __ffsll((long long)used) - 1 : -1;
+}
+// The entries (token * top_k + slot) of expert e in token order -- a token chooses an expert once: at most T -- and their number.  Every wave
+// writes the whole list (the same values) and so may read it without a barrier.
+__device__ __forceinline__ int entries_of(const int* idx, int n, int e, int lane, int* list) {
+    int count = 0;
+    for (int i0 = 0; i0 < n; i0 += 64) {
+        const bool hit = i0 + lane < n && idx[i0 + lane] == e;
+        const unsigned long long m = __ballot(hit);
+        if (hit) list[count + __popcll(m & ((1ull << lane) - 1ull))] = i0 + lane;
+        count += __popcll(m);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    return count;
 }
 
 // ------------------------------------------------------------------------------------------------------------- gate and up
-// Tokens of an expert are taken 16 MT at a time; a second pass finds the weights in the L2.
-template <typename A, int P, int MT, bool INSIDE>
-__global__ __launch_bounds__(64 * WAVES, (P == P_F32 || sizeof(A) == 2) ? 4 : 2) void few_up_kernel(const FewArgs a) {
+// A wave multiplies 16 NT gate rows and 16 NT up rows with 16 MT tokens over its part of the summed axis; `wk` waves share a group
+// of rows, WAVES / wk groups a workgroup.  Tokens of an expert are taken 16 MT at a time; a second pass finds the weights in the L2.
+// With many tokens NT = 2: every row group reads all tokens again from the L2, which costs as much as the weights at NT = 1
+// (64 tokens, width 1536, 8 experts of 6144: 85 us).
+template <typename A, int P, int MT, int NT, bool INSIDE>
+__global__ __launch_bounds__(64 * WAVES, P == P_F32 || sizeof(A) == 2 ? 4 : 2) void few_up_kernel(const FewArgs a) {
     typedef Weight<P> W;
     constexpr int CE = W::CE, PIECE = 8 * CE;                            // 128 bytes of a 16-bit or fp32 row
     constexpr bool RAW_X = P == P_F32 || sizeof(A) == 2;                 // token values go into the matrix instruction as they are
     constexpr int PX = RAW_X ? 1 : 3, PH = P == P_F32 ? 1 : sizeof(A) == 4 ? 3 : 2;
-    __shared__ float sums[WAVES][2 * MT][64][4];
+    __shared__ __attribute__((aligned(16))) float sums[WAVES][2 * MT * NT][64][4];
     __shared__ int idx_s[FEW_MAX_T * FEW_MAX_K];
     __shared__ float wts_s[INSIDE ? FEW_MAX_T * FEW_MAX_K : 1];
-    __shared__ Chosen ch;
+    __shared__ int list[FEW_MAX_T];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g = lane >> 4;
     const int n = a.T * a.top_k;
     if constexpr (INSIDE) {
-        static_assert(ROUTE_GROUPS * WAVES * 8 <= WAVES * 2 * 64 * 4, "the routing's sums fit");
-        route<A>(a, 0, a.T, &sums[0][0][0][0], idx_s, wts_s);
+        static_assert(ROUTE_TOKENS * ROUTE_WAVE <= WAVES * 2 * 64 * 4, "the routing's sums fit");
+        if (a.T == 1) route<A, 1>(a, 0, 1, &sums[0][0][0][0], idx_s, wts_s);
+        else
+            for (int t0 = 0; t0 < a.T; t0 += ROUTE_TOKENS)
+                route<A, ROUTE_TOKENS>(a, t0, min(ROUTE_TOKENS, a.T - t0), &sums[0][0][0][0], idx_s + t0 * a.top_k, wts_s + t0 * a.top_k);
         if (blockIdx.x == 0 && blockIdx.y == 0)
             for (int i = tid; i < n; i += 64 * WAVES) { a.idx[i] = idx_s[i]; a.wts[i] = wts_s[i]; }
     } else {
         for (int i = tid; i < n; i += 64 * WAVES) idx_s[i] = a.idx[i];
     }
-    if (blockIdx.x == 0 && blockIdx.y == 0 && a.shares > 1)
-        for (int i = tid; i < a.d / 16; i += 64 * WAVES) a.arrived[i] = 0;
     __syncthreads();
-    const int e = chosen_expert(idx_s, n, blockIdx.y, ch.used);
-    int* row_of_table = a.table + (int64_t)blockIdx.y * (a.T + 2);
-    if (e < 0) {
-        if (blockIdx.x == 0 && tid == 0) row_of_table[0] = -1;
-        return;
+    int chosen;
+    const int e = chosen_expert(idx_s, n, blockIdx.y, lane, &chosen);
+    int* row_of_table = a.table + 1 + (int64_t)blockIdx.y * (a.T + 2);
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+        if (tid == 0) a.table[0] = chosen;
+        for (int i = tid; i < a.arrivals; i += 64 * WAVES) a.arrived[i] = 0;
     }
-    entries_of(idx_s, n, e, ch);
-    const int count = ch.count, col0 = blockIdx.x * 16;
-    if (blockIdx.x == 0) {
-        if (tid < count) row_of_table[2 + tid] = ch.entry[tid];
+    if (e < 0) return;
+    const int count = entries_of(idx_s, n, e, lane, list);
+    if (blockIdx.x == 0 && wave == 0) {
+        if (lane < count) row_of_table[2 + lane] = list[lane];
         if (tid == 0) { row_of_table[0] = e; row_of_table[1] = count; }
     }
-    const int64_t low = (int64_t)a.E * 2 * a.inter * a.d;
-    const int64_t gate = ((int64_t)e * 2 * a.inter + col0 + r16) * a.d + g * CE, up = gate + (int64_t)a.inter * a.d;
+    const int col0 = ((int)blockIdx.x * (WAVES / a.wk) + wave / a.wk) * 16 * NT, kw = wave % a.wk;
+    // a wave-uniform base and 32-bit byte offsets a lane (the host limits an expert's matrix to 2^31 bytes)
+    const int64_t low = (int64_t)a.E * 2 * a.inter * a.d * W::SZ;
+    const unsigned char* gate = static_cast<const unsigned char*>(a.w13) + (int64_t)e * 2 * a.inter * a.d * W::SZ;
+    const unsigned char* up = gate + (int64_t)a.inter * a.d * W::SZ;
+    unsigned row[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) row[j] = ((unsigned)min(col0 + 16 * j + r16, a.inter - 1) * (unsigned)a.d + g * CE) * W::SZ;
     for (int m0 = 0; m0 < count; m0 += 16 * MT) {
-        const A* x[MT];
+        unsigned x[MT];
         bool live[MT];
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             live[t] = m0 + t * 16 + r16 < count;
-            x[t] = static_cast<const A*>(a.x) + (int64_t)(live[t] ? ch.entry[m0 + t * 16 + r16] / a.top_k : 0) * a.d + g * CE;
+            x[t] = ((unsigned)(live[t] ? list[m0 + t * 16 + r16] / a.top_k : 0) * (unsigned)a.d + g * CE) * sizeof(A);
         }
-        f32x4_t acc[2][MT];
+        f32x4_t acc[NT][2][MT];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) acc[0][t] = acc[1][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        constexpr int U = 2;                                              // pieces in flight a wave
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[j][0][t] = acc[j][1][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        constexpr int U = MT * NT > 1 ? 1 : 2;                            // pieces in flight a wave
         const int K = a.d - g * CE;
-        for (int k = wave * PIECE; k < a.d; k += U * WAVES * PIECE) {
-            W w[2 * U][2];
-            uint4 xv[2 * U][MT][RAW_X ? 1 : 2];
+        const int stride = U * a.wk * PIECE;
+        W w[2 * U][NT][2];
+        uint4 xv[2 * U][MT][RAW_X ? 1 : 2];
+        auto load = [&](int q, int k) {                                   // half piece q of the round that starts at k; zero past the end
+            const int kq = k + (q >> 1) * a.wk * PIECE + (q & 1) * 4 * CE;
+            const bool ok = kq < K;
 #pragma unroll
-            for (int q = 0; q < 2 * U; ++q) {
-                const int kq = k + (q >> 1) * WAVES * PIECE + (q & 1) * 4 * CE;
-                const bool ok = kq < K;
-                if (ok) { w[q][0].load(a.w13, gate + kq, low); w[q][1].load(a.w13, up + kq, low); }
-                else { w[q][0].clear(); w[q][1].clear(); }
-#pragma unroll
-                for (int t = 0; t < MT; ++t) {
-#pragma unroll
-                    for (int z = 0; z < (RAW_X ? 1 : 2); ++z)
-                        xv[q][t][z] = ok && live[t] ? *reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned char*>(x[t] + kq) + 16 * z) : make_uint4(0u, 0u, 0u, 0u);
-                }
+            for (int j = 0; j < NT; ++j) {
+                if (ok) { w[q][j][0].load(gate, row[j] + kq * W::SZ, low); w[q][j][1].load(up, row[j] + kq * W::SZ, low); }
+                else { w[q][j][0].clear(); w[q][j][1].clear(); }
             }
 #pragma unroll
-            for (int q = 0; q < 2 * U; ++q) {
+            for (int t = 0; t < MT; ++t) {
 #pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    if constexpr (P == P_F32) {
-                        acc[0][t] = mfma_f(w[q][0].raw[0], xv[q][t][0], acc[0][t]);
-                        acc[1][t] = mfma_f(w[q][1].raw[0], xv[q][t][0], acc[1][t]);
-                    } else if constexpr (RAW_X && P == P_BF16) {
-                        acc[0][t] = mfma_bf(w[q][0].raw[0], xv[q][t][0], acc[0][t]);
-                        acc[1][t] = mfma_bf(w[q][1].raw[0], xv[q][t][0], acc[1][t]);
-                    } else if constexpr (RAW_X) {
-                        acc[0][t] = mfma_h(w[q][0].raw[0], xv[q][t][0], acc[0][t]);
-                        acc[1][t] = mfma_h(w[q][1].raw[0], xv[q][t][0], acc[1][t]);
-                    } else {
+                for (int z = 0; z < (RAW_X ? 1 : 2); ++z)
+                    xv[q][t][z] = ok && live[t] ? *reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(a.x) + (unsigned)(x[t] + kq * sizeof(A) + 16 * z)) : make_uint4(0u, 0u, 0u, 0u);
+            }
+        };
+        for (int k = kw * PIECE; k < a.d; k += stride) {
+#pragma unroll
+            for (int q = 0; q < 2 * U; ++q) load(q, k);
+#pragma unroll
+            for (int q = 0; q < 2 * U; ++q) {
+                uint4 px[MT][PX];
+                if constexpr (!RAW_X) {
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
                         const float v[8] = {__uint_as_float(xv[q][t][0].x), __uint_as_float(xv[q][t][0].y), __uint_as_float(xv[q][t][0].z), __uint_as_float(xv[q][t][0].w),
                                             __uint_as_float(xv[q][t][1].x), __uint_as_float(xv[q][t][1].y), __uint_as_float(xv[q][t][1].z), __uint_as_float(xv[q][t][1].w)};
-                        uint4 px[PX], pw[W::PARTS];
-                        split8<PX>(v, px);
-#pragma unroll
-                        for (int z = 0; z < 2; ++z) {
-                            w[q][z].parts(pw);
-                            acc[z][t] = mfma_parts<W::PARTS, PX, 3>(pw, px, acc[z][t]);
-                        }
+                        split8<PX>(v, px[t]);
                     }
                 }
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        uint4 pw[W::PARTS];
+                        if constexpr (!RAW_X) w[q][j][z].parts(pw);
+#pragma unroll
+                        for (int t = 0; t < MT; ++t) {
+                            if constexpr (P == P_F32) acc[j][z][t] = mfma_f(w[q][j][z].raw[0], xv[q][t][0], acc[j][z][t]);
+                            else if constexpr (RAW_X && P == P_BF16) acc[j][z][t] = mfma_bf(w[q][j][z].raw[0], xv[q][t][0], acc[j][z][t]);
+                            else if constexpr (RAW_X) acc[j][z][t] = mfma_h(w[q][j][z].raw[0], xv[q][t][0], acc[j][z][t]);
+                            else acc[j][z][t] = mfma_parts<W::PARTS, PX, 3>(pw, px[t], acc[j][z][t]);
+                        }
+                    }
             }
         }
         __syncthreads();                                                  // what `sums` held before has been read
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            *reinterpret_cast<f32x4_t*>(sums[wave][2 * t][lane]) = acc[0][t];
-            *reinterpret_cast<f32x4_t*>(sums[wave][2 * t + 1][lane]) = acc[1][t];
-        }
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                *reinterpret_cast<f32x4_t*>(sums[wave][(j * MT + t) * 2][lane]) = acc[j][0][t];
+                *reinterpret_cast<f32x4_t*>(sums[wave][(j * MT + t) * 2 + 1][lane]) = acc[j][1][t];
+            }
         __syncthreads();
         // result layout of the 16x16 product: column (token) = lane & 15, row (hidden column) = 4 (lane >> 4) + reg
-        const int rows = min(count - m0, 16 * MT);
-        for (int i = tid; i < rows * 16; i += 64 * WAVES) {
-            const int m = i >> 4, c = i & 15, t = m >> 4, l = (c >> 2) * 16 + (m & 15);
+        const int rows = min(count - m0, 16 * MT), cols = 16 * NT * (WAVES / a.wk), left = (int)blockIdx.x * cols;
+        for (int i = tid; i < rows * cols; i += 64 * WAVES) {
+            const int m = i / cols, c = i - m * cols, w0 = c / (16 * NT) * a.wk, cc = c % (16 * NT);
+            if (left + c >= a.inter) continue;
+            const int t = ((cc >> 4) * MT + (m >> 4)) * 2, l = ((cc & 15) >> 2) * 16 + (m & 15);
             float vg = 0.f, vu = 0.f;
-#pragma unroll
-            for (int s = 0; s < WAVES; ++s) { vg += sums[s][2 * t][l][c & 3]; vu += sums[s][2 * t + 1][l][c & 3]; }
+            for (int s = 0; s < a.wk; ++s) { vg += sums[w0 + s][t][l][c & 3]; vu += sums[w0 + s][t + 1][l][c & 3]; }
             float v = vg / (1.f + expf(-vg)) * vu;
-            const int64_t at = (int64_t)ch.entry[m0 + m] * a.inter + col0 + c;
+            const int64_t at = (int64_t)list[m0 + m] * a.inter + left + c;
             if constexpr (P == P_F32) static_cast<float*>(a.h)[at] = v;
             else {
 #pragma unroll
@@ -372,161 +424,196 @@ __global__ __launch_bounds__(64 * WAVES, (P == P_F32 || sizeof(A) == 2) ? 4 : 2)
 }
 
 // ------------------------------------------------------------------------------------------------------------- down
-template <typename A, int P, int MT>
-__global__ __launch_bounds__(64 * WAVES, (P == P_F32 || sizeof(A) == 2) ? 4 : 2) void few_down_kernel(const FewArgs a) {
+// A workgroup multiplies 16 NT rows of one expert's matrix with that expert's hidden rows over one of k_splits parts of the hidden
+// axis (its waves share the part) and leaves the sums of every (token, slot) entry; the last workgroup of a group of output columns
+// adds a token's entries, weighted, slot by slot and part by part.
+template <typename A, int P, int MT, int NT>
+__global__ __launch_bounds__(64 * WAVES, P == P_F32 || (P == P_BF16 && sizeof(A) == 2) ? 4 : 2) void few_down_kernel(const FewArgs a) {
     typedef Weight<P> W;
-    constexpr int CE = W::CE, PIECE = 8 * CE, PH = P == P_F32 ? 1 : sizeof(A) == 4 ? 3 : 2;
-    constexpr int ROWS = MT == 1 ? 16 : FEW_MAX_T;                        // tokens the launch may have
-    __shared__ float ysum[WAVES][ROWS][16 + 1];
+    constexpr int CE = W::CE, PIECE = 8 * CE, PH = P == P_F32 ? 1 : sizeof(A) == 4 ? 3 : 2, COLS = 16 * NT;
+    __shared__ __attribute__((aligned(16))) float sums[WAVES][MT * NT][64][4];
     __shared__ int last;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g = lane >> 4;
-    const int col0 = blockIdx.x * 16;
-    for (int i = lane; i < ROWS * 17; i += 64) (&ysum[wave][0][0])[i] = 0.f;
-    __syncthreads();
-    const int64_t low = (int64_t)a.E * a.inter * a.d;
-    // unit u = (chosen expert u / k_splits, part u % k_splits of the hidden axis); this workgroup takes every shares-th
-    const int piece_len = (a.inter + a.k_splits * PIECE - 1) / (a.k_splits * PIECE) * PIECE;
-    for (int u = blockIdx.y; u < a.active * a.k_splits; u += a.shares) {
-        const int* row_of_table = a.table + (int64_t)(u / a.k_splits) * (a.T + 2);
-        const int e = row_of_table[0];
-        if (e < 0) break;
-        const int count = row_of_table[1], k_lo = (u % a.k_splits) * piece_len, k_hi = min(k_lo + piece_len, a.inter);
-        const int64_t row = ((int64_t)e * a.d + col0 + r16) * a.inter + g * CE;
-        for (int m0 = 0; m0 < count; m0 += 16 * MT) {
-            int64_t h[MT];
-            int entry[MT];
-            float wt[MT];
-            bool live[MT];
+    const int col0 = blockIdx.x * COLS, chosen = a.table[0], n = a.T * a.top_k;
+    const int rank = blockIdx.y / a.k_splits, part = blockIdx.y % a.k_splits;
+    if (rank >= chosen) return;
+    const int* row_of_table = a.table + 1 + (int64_t)rank * (a.T + 2);
+    const int e = row_of_table[0], count = row_of_table[1];
+    const int64_t low = (int64_t)a.E * a.inter * a.d * W::SZ;
+    const unsigned char* w2 = static_cast<const unsigned char*>(a.w2) + (int64_t)e * a.inter * a.d * W::SZ;
+    const unsigned char* hidden[PH];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                live[t] = m0 + t * 16 + r16 < count;
-                entry[t] = live[t] ? row_of_table[2 + m0 + t * 16 + r16] : 0;
-                wt[t] = a.wts[entry[t]];
-                h[t] = (int64_t)entry[t] * a.inter + g * CE;
+    for (int p = 0; p < PH; ++p) hidden[p] = static_cast<const unsigned char*>(a.h) + p * a.h_plane * W::SZ;
+    const int len = (a.inter + a.k_splits * PIECE - 1) / (a.k_splits * PIECE) * PIECE, k_lo = part * len, k_hi = min(k_lo + len, a.inter);
+    unsigned row[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) row[j] = ((unsigned)min(col0 + 16 * j + r16, a.d - 1) * (unsigned)a.inter + g * CE) * W::SZ;
+    for (int m0 = 0; m0 < count; m0 += 16 * MT) {
+        unsigned h[MT];
+        bool live[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int m = m0 + t * 16 + r16, entry = row_of_table[2 + min(m, a.T - 1)];     // read before `count` is known: one round trip
+            live[t] = m < count;
+            h[t] = ((unsigned)(live[t] ? entry : 0) * (unsigned)a.inter + g * CE) * W::SZ;
+        }
+        f32x4_t acc[NT][MT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[j][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        constexpr int REGS = NT * W::RAW + MT * PH, U = REGS <= 2 ? 4 : REGS <= 4 ? 2 : 1;    // pieces in flight a wave, by registers
+        const int K = k_hi - g * CE;
+        constexpr int STRIDE = U * WAVES * PIECE;
+        W w[2 * U][NT];
+        uint4 hv[2 * U][MT][PH];
+        auto load = [&](int q, int k) {                                   // half piece q of the round that starts at k; zero past the end
+            const int kq = k + (q >> 1) * WAVES * PIECE + (q & 1) * 4 * CE;
+            const bool ok = kq < K;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                if (ok) w[q][j].load(w2, row[j] + kq * W::SZ, low);
+                else w[q][j].clear();
             }
-            f32x4_t acc[MT];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-            constexpr int U = W::RAW + MT * PH > 4 ? 1 : W::RAW + MT * PH > 2 ? 2 : 4;    // pieces in flight a wave, by registers
-            const int K = k_hi - g * CE;
-            for (int k = k_lo + wave * PIECE; k < k_hi; k += U * WAVES * PIECE) {
-                W w[2 * U];
-                uint4 hv[2 * U][MT][PH];
+            for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int q = 0; q < 2 * U; ++q) {
-                    const int kq = k + (q >> 1) * WAVES * PIECE + (q & 1) * 4 * CE;
-                    const bool ok = kq < K;
-                    if (ok) w[q].load(a.w2, row + kq, low);
-                    else w[q].clear();
+                for (int p = 0; p < PH; ++p)
+                    hv[q][t][p] = ok && live[t] ? *reinterpret_cast<const uint4*>(hidden[p] + (unsigned)(h[t] + kq * W::SZ)) : make_uint4(0u, 0u, 0u, 0u);
+        };
+        for (int k = k_lo + wave * PIECE; k < k_hi; k += STRIDE) {
 #pragma unroll
-                    for (int t = 0; t < MT; ++t)
+            for (int q = 0; q < 2 * U; ++q) load(q, k);
 #pragma unroll
-                        for (int p = 0; p < PH; ++p)
-                            hv[q][t][p] = ok && live[t] ? *reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(a.h) + (p * a.h_plane + h[t] + kq) * W::SZ)
-                                                        : make_uint4(0u, 0u, 0u, 0u);
-                }
+            for (int q = 0; q < 2 * U; ++q) {
 #pragma unroll
-                for (int q = 0; q < 2 * U; ++q) {
+                for (int j = 0; j < NT; ++j) {
                     uint4 pw[W::PARTS];
-                    if constexpr (P != P_F32) w[q].parts(pw);
+                    if constexpr (P != P_F32) w[q][j].parts(pw);
 #pragma unroll
                     for (int t = 0; t < MT; ++t) {
-                        if constexpr (P == P_F32) acc[t] = mfma_f(w[q].raw[0], hv[q][t][0], acc[t]);
-                        else acc[t] = mfma_parts<W::PARTS, PH, PH>(pw, hv[q][t], acc[t]);
+                        if constexpr (P == P_F32) acc[j][t] = mfma_f(w[q][j].raw[0], hv[q][t][0], acc[j][t]);
+                        else acc[j][t] = mfma_parts<W::PARTS, PH, PH>(pw, hv[q][t], acc[j][t]);
                     }
                 }
             }
-            // a token chooses an expert once: the lanes of a wave add to different rows
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-                if (live[t]) {
-                    const int tok = entry[t] / a.top_k;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) ysum[wave][tok][4 * g + q] += wt[t] * acc[t][q];
-                }
         }
-    }
-    __syncthreads();
-    const A* res = static_cast<const A*>(a.res);
-    A* y = static_cast<A*>(a.y);
-    if (a.shares == 1) {
-        for (int i = tid; i < a.T * 16; i += 64 * WAVES) {
-            const int t = i >> 4, c = i & 15;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) *reinterpret_cast<f32x4_t*>(sums[wave][j * MT + t][lane]) = acc[j][t];
+        __syncthreads();
+        const int rows = min(count - m0, 16 * MT);
+        for (int i = tid; i < rows * COLS; i += 64 * WAVES) {
+            const int m = i / COLS, c = i % COLS;
+            if (col0 + c >= a.d) continue;
+            const int t = (c >> 4) * MT + (m >> 4), l = ((c & 15) >> 2) * 16 + (m & 15);
             float v = 0.f;
 #pragma unroll
-            for (int s = 0; s < WAVES; ++s) v += ysum[s][t][c];
-            const int64_t at = (int64_t)t * a.d + col0 + c;
-            if (res) v += (float)res[at];
-            y[at] = (A)v;
+            for (int s = 0; s < WAVES; ++s) v += sums[s][t][l][c & 3];
+            __hip_atomic_store(&a.part[((int64_t)part * n + row_of_table[2 + m0 + m]) * a.d + col0 + c], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        return;
     }
-    for (int i = tid; i < a.T * 16; i += 64 * WAVES) {
-        const int t = i >> 4, c = i & 15;
-        float v = 0.f;
-#pragma unroll
-        for (int s = 0; s < WAVES; ++s) v += ysum[s][t][c];
-        __hip_atomic_store(&a.part[((int64_t)blockIdx.y * a.T + t) * a.d + col0 + c], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    // The last workgroup of this column group adds the shares.  Nobody waits: the others have left.  The shares are written and read
-    // by device-scope accesses, which go past the L2 of an XCD; every wave waits for its own to arrive before the workgroup is counted.
+    // The last workgroup of this column group joins.  Nobody waits: the others have left.  The sums are written and read by device-scope
+    // accesses, which go past the L2 of an XCD; every wave waits for its own to arrive before the workgroup is counted.
     // (A device-scope fence does the same by writing back the whole L2: 40 us for one token of width 512.)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (tid == 0) last = __hip_atomic_fetch_add(&a.arrived[blockIdx.x], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.shares - 1;
+    if (tid == 0) last = __hip_atomic_fetch_add(&a.arrived[blockIdx.x], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == chosen * a.k_splits - 1;
     __syncthreads();
     if (!last) return;
-    for (int i = tid; i < a.T * 16; i += 64 * WAVES) {
-        const int t = i >> 4, c = i & 15;
-        const int64_t at = (int64_t)t * a.d + col0 + c;
-        float v = res ? (float)res[at] : 0.f;
-        float s = 0.f;
-        for (int p0 = 0; p0 < a.shares; p0 += 8) {                        // eight loads in flight, added in order
-            float f[8];
+    // Two columns an item, two items and eight terms at a time: a thread's loads are in flight together, for the tail of the launch is their latency.
+    const A* res = static_cast<const A*>(a.res);
+    const int terms = a.top_k * a.k_splits, items = a.T * (COLS / 2);
+    typedef unsigned long long u64;
+    constexpr int J = 2, C = 8;
+    for (int i0 = tid; i0 < items; i0 += J * 64 * WAVES) {
+        float s0[J], s1[J];
+        int t[J], c[J];
 #pragma unroll
-            for (int p = 0; p < 8; ++p) f[p] = __hip_atomic_load(&a.part[(int64_t)min(p0 + p, a.shares - 1) * a.T * a.d + at], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-            for (int p = 0; p < 8; ++p) s += p0 + p < a.shares ? f[p] : 0.f;
+        for (int j = 0; j < J; ++j) {
+            const int i = min(i0 + j * 64 * WAVES, items - 1);
+            t[j] = i / (COLS / 2);
+            c[j] = min(col0 + i % (COLS / 2) * 2, a.d - 2);               // columns behind d repeat the last two
+            s0[j] = s1[j] = 0.f;
         }
-        y[at] = (A)(s + v);
+        for (int q0 = 0; q0 < terms; q0 += C) {
+            u64 f[J][C];
+            float wt[J][C];
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int p = 0; p < C; ++p) {
+                    const int q = min(q0 + p, terms - 1), slot = q / a.k_splits, entry = t[j] * a.top_k + slot;
+                    wt[j][p] = a.wts[entry];
+                    f[j][p] = __hip_atomic_load(reinterpret_cast<const u64*>(a.part + ((int64_t)(q - slot * a.k_splits) * n + entry) * a.d + c[j]), __ATOMIC_RELAXED,
+                                                __HIP_MEMORY_SCOPE_AGENT);
+                }
+#pragma unroll
+            for (int p = 0; p < C; ++p)
+                if (q0 + p < terms) {
+#pragma unroll
+                    for (int j = 0; j < J; ++j) {
+                        s0[j] += wt[j][p] * __uint_as_float((unsigned)f[j][p]);
+                        s1[j] += wt[j][p] * __uint_as_float((unsigned)(f[j][p] >> 32));
+                    }
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            if (i0 + j * 64 * WAVES >= items) break;
+            const int64_t at = (int64_t)t[j] * a.d + c[j];
+            Pack<A, 2> r, o;
+            if (res) r = *reinterpret_cast<const Pack<A, 2>*>(res + at);
+            o.v[0] = (A)(s0[j] + (res ? (float)r.v[0] : 0.f));
+            o.v[1] = (A)(s1[j] + (res ? (float)r.v[1] : 0.f));
+            *reinterpret_cast<Pack<A, 2>*>(static_cast<A*>(a.y) + at) = o;
+        }
     }
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
 inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-struct FewPlan { int shares, k_splits, active; size_t idx, wts, table, h, part, arrived, bytes; int64_t h_plane; };
+// Row groups of a wave: one while the tokens fit one matrix tile, else as many as make the tokens' reads small against the weights'
+inline int up_nt(int T) { return T <= 16 ? 1 : 2; }
+inline int down_nt(int T) { return T <= 16 ? 1 : 4; }
+
+struct FewPlan { int active, wk, up_blocks, k_splits, down_blocks; size_t idx, wts, table, h, part, arrived, bytes; int64_t h_plane; };
 
 FewPlan few_plan(int T, int d, int inter, int E, int top_k, int act_type, int precision) {
     FewPlan p;
     const int n = T * top_k, piece = precision == P_F32 ? 32 : 64;
     p.active = n < E ? n : E;                                             // experts that can have been chosen
-    // enough workgroups to keep the whole card loading, each with at least a piece of the hidden axis for every wave
-    const int groups = d / 16;
-    int want = (512 + groups - 1) / groups;
-    const int most_k = inter / (piece * WAVES) > 1 ? inter / (piece * WAVES) : 1;
-    p.k_splits = 1;
-    if (want > p.active) p.k_splits = (want + p.active - 1) / p.active;
-    if (p.k_splits > most_k) p.k_splits = most_k;
-    // as many units each: an uneven share is a second round for all
-    const int units = p.active * p.k_splits, per = units > want ? units / want : 1;
-    p.shares = (units + per - 1) / per;
+    // Both products: two workgroups a CU at most where that leaves none idle -- a workgroup more is a second round for all.
+    // `up`: by the number of waves that share a row group ...
+    const int groups = (inter + 16 * up_nt(T) - 1) / (16 * up_nt(T));
+    p.wk = WAVES;
+    while (p.wk > 1 && (groups + WAVES / p.wk - 1) / (WAVES / p.wk) * p.active > UP_BLOCKS) p.wk /= 2;
+    p.up_blocks = (groups + WAVES / p.wk - 1) / (WAVES / p.wk);
+    // ... `down`: by the number of parts of the hidden axis, each with a piece for every wave
+    p.down_blocks = (d + 16 * down_nt(T) - 1) / (16 * down_nt(T));
+    const int64_t bytes = (int64_t)p.active * d * inter * (precision == P_F32 ? 4 : 2) / DOWN_KB >> 10;
+    const int want = (int)((bytes > DOWN_BLOCKS ? bytes : DOWN_BLOCKS) / (p.down_blocks * p.active)), most = inter / (piece * WAVES);
+    p.k_splits = want < most ? want : most;
+    if (p.k_splits < 1) p.k_splits = 1;
     p.h_plane = (int64_t)n * inter;
     size_t off = 0;
     auto take = [&](size_t b) { const size_t at = off; off += up256(b); return at; };
     p.idx = take((size_t)n * 4);
     p.wts = take((size_t)n * 4);
-    p.table = take((size_t)p.active * (T + 2) * 4);
+    p.table = take((1 + (size_t)p.active * (T + 2)) * 4);
     p.h = take((size_t)p.h_plane * (precision == P_F32 ? 4 : act_type == DT_F32 ? 6 : 4));
-    p.part = take(p.shares > 1 ? (size_t)p.shares * T * d * 4 : 0);
-    p.arrived = take((size_t)groups * 4);
+    p.part = take((size_t)p.k_splits * n * d * 4);
+    p.arrived = take((size_t)p.down_blocks * 4);
     p.bytes = off;
     return p;
 }
 
 bool few_shape_ok(int T, int d, int inter, int E, int top_k) {
     return T >= 1 && T <= FEW_MAX_T && d >= 32 && d % 32 == 0 && d <= (1 << 16) && inter >= 32 && inter % 32 == 0 && inter <= (1 << 18) && E >= 1 && E <= FEW_MAX_E && top_k >= 1 &&
-           top_k <= FEW_MAX_K && top_k <= E;
+           top_k <= FEW_MAX_K && top_k <= E && (int64_t)d * inter <= 1 << 28;
 }
 
 bool few_types_ok(int act_type, int precision) {
@@ -534,26 +621,27 @@ bool few_types_ok(int act_type, int precision) {
     return (act_type == DT_BF16 && precision == P_BF16) || (act_type == DT_F16 && precision == P_F16);
 }
 
-// tokens times groups of eight experts up to which `up` routes by itself
-constexpr int ROUTE_INSIDE = 2;
-static_assert(ROUTE_INSIDE <= ROUTE_GROUPS, "fits LDS");
-
-template <typename A, int P, int MT>
+// Tokens up to which `up` routes by itself: as long as all fit one round (the launch it saves costs 4 us, a second round 5)
+constexpr int ROUTE_INSIDE = ROUTE_TOKENS;
+template <typename A, int P, int MT, int UP_NT, int DOWN_NT>
 void launch_few_layer(const FewArgs& a, const FewPlan& p, hipStream_t s) {
-    const dim3 up((unsigned)(a.inter / 16), (unsigned)p.active), down((unsigned)(a.d / 16), (unsigned)p.shares), block(64 * WAVES);
-    if (a.T * ((a.E + 7) / 8) <= ROUTE_INSIDE) {
-        hipLaunchKernelGGL((few_up_kernel<A, P, MT, true>), up, block, 0, s, a);
-    } else {
-        hipLaunchKernelGGL(few_route_kernel<A>, dim3((unsigned)a.T), block, 0, s, a);
-        hipLaunchKernelGGL((few_up_kernel<A, P, MT, false>), up, block, 0, s, a);
+    const dim3 up((unsigned)p.up_blocks, (unsigned)p.active), down((unsigned)p.down_blocks, (unsigned)(p.active * p.k_splits)), block(64 * WAVES);
+    bool inside = false;
+    if constexpr (MT == 1) {
+        inside = a.T <= ROUTE_INSIDE;
+        if (inside) hipLaunchKernelGGL((few_up_kernel<A, P, 1, UP_NT, true>), up, block, 0, s, a);
     }
-    hipLaunchKernelGGL((few_down_kernel<A, P, MT>), down, block, 0, s, a);
+    if (!inside) {
+        hipLaunchKernelGGL(few_route_kernel<A>, dim3((unsigned)a.T), block, 0, s, a);
+        hipLaunchKernelGGL((few_up_kernel<A, P, MT, UP_NT, false>), up, block, 0, s, a);
+    }
+    hipLaunchKernelGGL((few_down_kernel<A, P, MT, DOWN_NT>), down, block, 0, s, a);
 }
 
 template <typename A, int P>
 void launch_by_tokens(const FewArgs& a, const FewPlan& p, hipStream_t s) {
-    if (a.T <= 16) launch_few_layer<A, P, 1>(a, p, s);
-    else launch_few_layer<A, P, 2>(a, p, s);
+    if (a.T <= 16) launch_few_layer<A, P, 1, 1, 1>(a, p, s);
+    else launch_few_layer<A, P, 2, 2, 4>(a, p, s);
 }
 
 }  // namespace
@@ -572,7 +660,7 @@ ADX_API int adx_op_moe_few(const void* x, const void* res, const float* router_w
                            int top_k, int act_type, int precision, void* workspace, size_t workspace_bytes, void* y, void* stream) {
     if (!x || !router_w || !w13 || !w2 || !workspace || !y) { set_error("moe_few: null pointer"); return ADX_EINVAL; }
     if (!few_shape_ok(T, d, inter, E, top_k)) {
-        set_error("moe_few: needs 1 <= T <= 64 tokens, 1 <= top_k <= min(E, 8), E <= 64, and hidden (<= 65536) / expert (<= 262144) widths that are multiples of 32"); return ADX_EINVAL;
+        set_error("moe_few: needs 1 <= T <= 64 tokens, 1 <= top_k <= min(E, 8), E <= 64, and hidden (<= 65536) / expert (<= 262144) widths that are multiples of 32 with d * inter <= 2^28"); return ADX_EINVAL;
     }
     if (!few_types_ok(act_type, precision)) {
         set_error("moe_few: fp32 tokens with fp32, bf16, bf16x3 or f16 weights, bf16 tokens with bf16 weights, fp16 tokens with f16 weights"); return ADX_EINVAL;
@@ -587,9 +675,9 @@ ADX_API int adx_op_moe_few(const void* x, const void* res, const float* router_w
     FewArgs a;
     a.x = x; a.res = res; a.router = router_w; a.w13 = w13; a.w2 = w2; a.T = T; a.d = d; a.inter = inter; a.E = E; a.top_k = top_k;
     a.idx = reinterpret_cast<int*>(base + p.idx); a.wts = reinterpret_cast<float*>(base + p.wts);
-    a.table = reinterpret_cast<int*>(base + p.table); a.active = p.active;
+    a.table = reinterpret_cast<int*>(base + p.table);
     a.h = base + p.h; a.h_plane = p.h_plane; a.part = reinterpret_cast<float*>(base + p.part); a.arrived = reinterpret_cast<int*>(base + p.arrived);
-    a.shares = p.shares; a.k_splits = p.k_splits; a.y = y;
+    a.arrivals = p.down_blocks; a.wk = p.wk; a.k_splits = p.k_splits; a.y = y;
     hipStream_t s = (hipStream_t)stream;
     if (act_type == DT_BF16) launch_by_tokens<__bf16, P_BF16>(a, p, s);
     else if (act_type == DT_F16) launch_by_tokens<_Float16, P_F16>(a, p, s);
