@@ -35,73 +35,69 @@ __device__ __forceinline__ float sigmoid_fast(float z) { return rcp_fast(1.f + e
 // z + 0.044715 z^3 scaled so that its sigmoid is (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2
 __device__ __forceinline__ float gelu_tanh_arg(float z) { return 1.59576912160573071f * z * (1.f + 0.044715f * z * z); }
 
-template <int V> __device__ __forceinline__ void apply_act(float (&v)[V], int act) {
+// act(z) in place and, with SLOPE, act'(z) from the same exponentials
+template <int V, bool SLOPE> __device__ __forceinline__ void apply_act(float (&v)[V], float (&d)[V], int act) {
     switch (act) {                                                 // uniform: one branch for all values
         case ACT_RELU:
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];          // NaN stays
+            for (int e = 0; e < V; ++e) { if (SLOPE) d[e] = v[e] > 0.f ? 1.f : v[e] == v[e] ? 0.f : v[e]; v[e] = v[e] < 0.f ? 0.f : v[e]; }      // NaN stays
             break;
         case ACT_LEAKY:
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = v[e] > 0.f ? v[e] : 0.01f * v[e];
+            for (int e = 0; e < V; ++e) { if (SLOPE) d[e] = v[e] > 0.f ? 1.f : v[e] == v[e] ? 0.01f : v[e]; v[e] = v[e] > 0.f ? v[e] : 0.01f * v[e]; }
             break;
         case ACT_SILU:
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] *= sigmoid_fast(v[e]);
+            for (int e = 0; e < V; ++e) { const float g = sigmoid_fast(v[e]); if (SLOPE) d[e] = g * (1.f + v[e] * (1.f - g)); v[e] *= g; }
             break;
         case ACT_TANH_:
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = tanhf(v[e]);
-            break;
-        case ACT_GELU_ERF:
-#pragma unroll
-            for (int e = 0; e < V; ++e) { const float q = normal_tail(v[e]); v[e] *= v[e] > 0.f ? 1.f - q : q; }
-            break;
-        case ACT_GELU_TANH:
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[e] *= sigmoid_fast(gelu_tanh_arg(v[e]));
-            break;
-        default: break;
-    }
-}
-
-template <int V> __device__ __forceinline__ void act_slopes(const float (&z)[V], float (&d)[V], int act) {
-    switch (act) {
-        case ACT_RELU:
-#pragma unroll
-            for (int e = 0; e < V; ++e) d[e] = z[e] > 0.f ? 1.f : 0.f;
-            break;
-        case ACT_LEAKY:
-#pragma unroll
-            for (int e = 0; e < V; ++e) d[e] = z[e] > 0.f ? 1.f : 0.01f;
-            break;
-        case ACT_SILU:
-#pragma unroll
-            for (int e = 0; e < V; ++e) { const float g = sigmoid_fast(z[e]); d[e] = g * (1.f + z[e] * (1.f - g)); }
-            break;
-        case ACT_TANH_:
-#pragma unroll
-            for (int e = 0; e < V; ++e) { const float t = tanhf(z[e]); d[e] = 1.f - t * t; }
+            for (int e = 0; e < V; ++e) { v[e] = tanhf(v[e]); if (SLOPE) d[e] = 1.f - v[e] * v[e]; }
             break;
         case ACT_GELU_ERF:
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float q = normal_tail(z[e]);
-                d[e] = (z[e] > 0.f ? 1.f - q : q) + z[e] * 0.39894228040143268f * exp2_fast(-0.72134752044448170f * z[e] * z[e]);
+                const float q = normal_tail(v[e]), p = v[e] > 0.f ? 1.f - q : q;
+                if (SLOPE) d[e] = p + v[e] * 0.39894228040143268f * exp2_fast(-0.72134752044448170f * v[e] * v[e]);
+                v[e] *= p;
             }
             break;
         case ACT_GELU_TANH:
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float c = fminf(fmaxf(z[e], -30.f), 30.f), g = sigmoid_fast(gelu_tanh_arg(c));      // beyond 30 the slope is 0 or 1
-                d[e] = g + c * g * (1.f - g) * 1.59576912160573071f * (1.f + 0.134145f * c * c);
-                if (z[e] != z[e]) d[e] = z[e];
+                const float g = sigmoid_fast(gelu_tanh_arg(v[e]));
+                if (SLOPE) {
+                    const float c = fminf(fmaxf(v[e], -30.f), 30.f);            // beyond 30 the slope is 0 or 1
+                    d[e] = v[e] == v[e] ? g + c * g * (1.f - g) * 1.59576912160573071f * (1.f + 0.134145f * c * c) : v[e];
+                }
+                v[e] *= g;
             }
             break;
         default:
+            if (SLOPE)
 #pragma unroll
-            for (int e = 0; e < V; ++e) d[e] = 1.f;
+                for (int e = 0; e < V; ++e) d[e] = 1.f;
     }
+}
+
+// What the forward keeps for the gradient is the activation's slope, not its argument: the backward needs no exponentials, and in 16
+// bits a slope (-0.13 .. 1.13) fits to 2^-16 as a fixed-point number, where an argument rounded to bf16 moves the gradient as much
+// as the rounding of dz does.  fp32 tensors keep it as it is.  Codes: (q - 8192) / 32768, 65535 for NaN, the piecewise activations 1 where
+// the argument is positive.
+template <typename T> struct Slope { typedef unsigned short type; };
+template <> struct Slope<float> { typedef float type; };
+__device__ __forceinline__ float slope_code(float d, int act, float) { return d; }
+__device__ __forceinline__ unsigned short slope_code(float d, int act, unsigned short) {
+    if (d != d) return 65535;
+    if (act == ACT_RELU || act == ACT_LEAKY) return d == 1.f;
+    return (unsigned short)(int)rintf(d * 32768.f + 8192.f);
+}
+__device__ __forceinline__ float slope_value(float q, int act) { return q; }
+__device__ __forceinline__ float slope_value(unsigned short q, int act) {
+    if (q == 65535) return __builtin_nanf("");
+    if (act == ACT_RELU) return (float)q;
+    if (act == ACT_LEAKY) return q ? 1.f : 0.01f;
+    return (float)((int)q - 8192) * (1.f / 32768.f);
 }
 
 // ------------------------------------------------------------------------------------------------------------- the problem
@@ -110,7 +106,7 @@ struct ProductArgs {
     const void* B; int64_t ldb;
     int64_t M; int N; int64_t K;             // C is M x N, K is summed
     const void* bias; const void* res; int64_t ldr;
-    void* pre;                               // [M][N]: the value before the activation (for the gradient)
+    void* slope;                             // [M][N]: the activation's slope (for the gradient), Slope<T>
     void* y; int64_t ldy;
     int act;
     int splits; int64_t k_split;             // K range of one split (a multiple of the K step)
@@ -122,43 +118,43 @@ struct ProductArgs {
 // V consecutive columns of one row: bias, activation, residual, one rounding, store
 template <typename T, int V>
 __device__ __forceinline__ void finish(const ProductArgs& a, int64_t m, int n, float (&v)[V], bool vec) {
+    typedef typename Slope<T>::type S;
     T* y = static_cast<T*>(a.y) + m * a.ldy + n;
     const T* bias = static_cast<const T*>(a.bias);
     const T* res = static_cast<const T*>(a.res) + (a.res ? m * a.ldr + n : 0);
-    T* pre = static_cast<T*>(a.pre) + (a.pre ? m * a.N + n : 0);
+    S* slope = static_cast<S*>(a.slope) + (a.slope ? m * a.N + n : 0);
     typedef Pack<T, V> P;
+    float d[V];
     if (vec) {
         if (bias) {
             const P b = *reinterpret_cast<const P*>(bias + n);
 #pragma unroll
             for (int e = 0; e < V; ++e) v[e] += (float)b.v[e];
         }
-        P o;
-        if (a.pre) {
+        if (a.slope) {
+            apply_act<V, true>(v, d, a.act);
+            Pack<S, V> q;
 #pragma unroll
-            for (int e = 0; e < V; ++e) o.v[e] = (T)v[e];
-            *reinterpret_cast<P*>(pre) = o;
-        }
-        apply_act<V>(v, a.act);
+            for (int e = 0; e < V; ++e) q.v[e] = slope_code(d[e], a.act, S());
+            *reinterpret_cast<Pack<S, V>*>(slope) = q;
+        } else apply_act<V, false>(v, d, a.act);
         if (a.res) {
             const P r = *reinterpret_cast<const P*>(res);
 #pragma unroll
             for (int e = 0; e < V; ++e) v[e] += (float)r.v[e];
         }
+        P o;
 #pragma unroll
         for (int e = 0; e < V; ++e) o.v[e] = (T)v[e];
         *reinterpret_cast<P*>(y) = o;
     } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            if (n + e >= a.N) break;
-            if (bias) v[e] += (float)bias[n + e];
-            if (a.pre) pre[e] = (T)v[e];
-        }
-        apply_act<V>(v, a.act);
+        for (int e = 0; e < V; ++e) if (bias && n + e < a.N) v[e] += (float)bias[n + e];
+        apply_act<V, true>(v, d, a.act);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             if (n + e >= a.N) break;
+            if (a.slope) slope[e] = slope_code(d[e], a.act, S());
             if (a.res) v[e] += (float)res[e];
             y[e] = (T)v[e];
         }
@@ -591,8 +587,9 @@ __global__ __launch_bounds__(64 * NWAVES) void product_few_kernel(const ProductA
 constexpr int SLOPE_ROWS = 64;
 
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void slope_kernel(const void* dy_, int64_t ldd, const void* pre_, void* dz_, float* part, int64_t M, int N, int act) {
+__global__ __launch_bounds__(256) void slope_kernel(const void* dy_, int64_t ldd, const void* slope_, void* dz_, float* part, int64_t M, int N, int act) {
     constexpr int V = VEC ? 16 / sizeof(T) : 1;
+    typedef typename Slope<T>::type S;
     __shared__ float sums[4][64 * V];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = (blockIdx.x * 64 + lane) * V;
@@ -602,18 +599,15 @@ __global__ __launch_bounds__(256) void slope_kernel(const void* dy_, int64_t ldd
 #pragma unroll
     for (int e = 0; e < V; ++e) sum[e] = 0.f;
     if (n < N) {
+#pragma unroll 4
         for (int64_t m = r0 + wave; m < r1; m += 4) {
             const P d = *reinterpret_cast<const P*>(static_cast<const T*>(dy_) + m * ldd + n);
-            P o;
             if (act != ACT_NONE) {
-                const P z = *reinterpret_cast<const P*>(static_cast<const T*>(pre_) + m * N + n);
-                float zv[V], sl[V];
-#pragma unroll
-                for (int e = 0; e < V; ++e) zv[e] = (float)z.v[e];
-                act_slopes<V>(zv, sl, act);
+                const Pack<S, V> q = *reinterpret_cast<const Pack<S, V>*>(static_cast<const S*>(slope_) + m * N + n);
+                P o;
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    const float g = (float)d.v[e] * sl[e];
+                    const float g = (float)d.v[e] * slope_value(q.v[e], act);
                     sum[e] += g;
                     o.v[e] = (T)g;
                 }
@@ -634,16 +628,24 @@ __global__ __launch_bounds__(256) void slope_kernel(const void* dy_, int64_t ldd
     }
 }
 
+constexpr int JOIN_WAVES = 16;
 template <typename T>
-__global__ __launch_bounds__(256) void colsum_join_kernel(const float* part, int64_t chunks, int N, void* out) {
-    __shared__ float sums[4][64];
+__global__ __launch_bounds__(64 * JOIN_WAVES) void colsum_join_kernel(const float* part, int64_t chunks, int N, void* out) {
+    __shared__ float sums[JOIN_WAVES][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = blockIdx.x * 64 + lane;
     float s = 0.f;
-    if (n < N)
-        for (int64_t c = wave; c < chunks; c += 4) s += part[c * N + n];
+    if (n < N) {
+#pragma unroll 4
+        for (int64_t c = wave; c < chunks; c += JOIN_WAVES) s += part[c * N + n];
+    }
     sums[wave][lane] = s;
     __syncthreads();
-    if (wave == 0 && n < N) static_cast<T*>(out)[n] = (T)((sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]));
+    if (wave == 0 && n < N) {
+        s = 0.f;
+#pragma unroll
+        for (int w = 0; w < JOIN_WAVES; ++w) s += sums[w][lane];
+        static_cast<T*>(out)[n] = (T)s;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
@@ -691,7 +693,7 @@ inline bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) =
 hipError_t product(ProductArgs a, int dt, bool acol, bool bcol, void* part, hipStream_t s) {
     const int V = 16 / dtype_bytes(dt);
     Plan p = plan_product(a.M, a.N, a.K, dt, acol, bcol);
-    a.vec = a.N % V == 0 && a.ldy % V == 0 && on16(a.y) && on16(a.bias) && (!a.res || (on16(a.res) && a.ldr % V == 0)) && on16(a.pre);
+    a.vec = a.N % V == 0 && a.ldy % V == 0 && on16(a.y) && on16(a.bias) && (!a.res || (on16(a.res) && a.ldr % V == 0)) && on16(a.slope);
     // operands by 16-byte pieces: rows start on 16 bytes and whole pieces make up the contiguous axis
     const bool pieces = on16(a.A) && on16(a.B) && a.lda % V == 0 && a.ldb % V == 0 && (acol ? a.M : a.K) % V == 0 && (bcol ? a.N : a.K) % V == 0;
     const bool near = a.lda < (1 << 21) && a.ldb < (1 << 21);  // a tile's 256 rows span less than 2^31 bytes
@@ -759,7 +761,7 @@ ADX_API size_t adx_linear_residual_ws_bytes(int64_t M, int N, int K, int dtype) 
     return plan_product(M, N, K, dtype, false, false).part_bytes;
 }
 
-ADX_API int adx_op_linear_residual(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldr, void* pre,
+ADX_API int adx_op_linear_residual(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldr, void* slope,
                                    void* y, int64_t ldy, int64_t M, int N, int K, int act, int dtype, void* workspace, size_t workspace_bytes,
                                    void* stream) {
     if (!dtype_ok(dtype)) { set_error("linear_residual: unknown element type"); return ADX_EINVAL; }
@@ -773,7 +775,7 @@ ADX_API int adx_op_linear_residual(const void* x, int64_t ldx, const void* w, in
         set_error("linear_residual: needs a 16-byte aligned workspace of adx_linear_residual_ws_bytes bytes"); return ADX_EINVAL;
     }
     ProductArgs a{};
-    a.A = x; a.lda = ldx; a.B = w; a.ldb = ldw; a.M = M; a.N = N; a.K = K; a.bias = bias; a.res = res; a.ldr = ldr; a.pre = pre; a.y = y; a.ldy = ldy;
+    a.A = x; a.lda = ldx; a.B = w; a.ldb = ldw; a.M = M; a.N = N; a.K = K; a.bias = bias; a.res = res; a.ldr = ldr; a.slope = slope; a.y = y; a.ldy = ldy;
     a.act = act;
     const hipError_t e = product(a, dtype, false, false, workspace, (hipStream_t)stream);
     return e == hipSuccess ? ADX_OK : hip_fail(e, "linear_residual");
@@ -784,13 +786,13 @@ ADX_API size_t adx_linear_residual_bwd_ws_bytes(int64_t M, int N, int K, int act
     return bwd_workspace(M, N, K, act, dtype).bytes;
 }
 
-ADX_API int adx_op_linear_residual_bwd(const void* dy, int64_t ldd, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* pre, void* dx,
+ADX_API int adx_op_linear_residual_bwd(const void* dy, int64_t ldd, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* slope, void* dx,
                                        void* dw, void* db, int64_t M, int N, int K, int act, int dtype, void* workspace, size_t workspace_bytes,
                                        void* stream) {
     if (!dtype_ok(dtype)) { set_error("linear_residual_bwd: unknown element type"); return ADX_EINVAL; }
     if (act < ACT_NONE || act > ACT_TANH_) { set_error("linear_residual_bwd: unknown activation"); return ADX_EINVAL; }
     if (!shape_ok(M, N, K) || M == 0) { set_error("linear_residual_bwd: needs 1 <= M <= 2^30 and positive N, K"); return ADX_EINVAL; }
-    if (!dy || (dx && !w) || (dw && !x) || (act != ACT_NONE && !pre)) { set_error("linear_residual_bwd: null pointer"); return ADX_EINVAL; }
+    if (!dy || (dx && !w) || (dw && !x) || (act != ACT_NONE && !slope)) { set_error("linear_residual_bwd: null pointer"); return ADX_EINVAL; }
     if (ldd < 0 || ldx < 0 || ldw < 0) { set_error("linear_residual_bwd: negative row stride"); return ADX_EINVAL; }
     const BwdWorkspace ws = bwd_workspace(M, N, K, act, dtype);
     if (!workspace || workspace_bytes < ws.bytes || !on16(workspace)) {
@@ -803,14 +805,14 @@ ADX_API int adx_op_linear_residual_bwd(const void* dy, int64_t ldd, const void* 
     const int V = 16 / dtype_bytes(dtype);
     if (act != ACT_NONE || db) {
         if (ws.chunks > 65535) { set_error("linear_residual_bwd: more than 4 million rows"); return ADX_EINVAL; }
-        const bool vec = N % V == 0 && ldd % V == 0 && on16(dy) && on16(pre);
+        const bool vec = N % V == 0 && ldd % V == 0 && on16(dy) && on16(slope);
         with_dtype(dtype, [&](auto t) {
             typedef decltype(t) T;
             const int cols = vec ? 64 * V : 64;
             const dim3 grid((unsigned)((N + cols - 1) / cols), (unsigned)ws.chunks);
-            if (vec) hipLaunchKernelGGL((slope_kernel<T, true>), grid, dim3(256), 0, s, dy, ldd, pre, dz, db ? sums : nullptr, M, N, act);
-            else hipLaunchKernelGGL((slope_kernel<T, false>), grid, dim3(256), 0, s, dy, ldd, pre, dz, db ? sums : nullptr, M, N, act);
-            if (db) hipLaunchKernelGGL(colsum_join_kernel<T>, dim3((unsigned)((N + 63) / 64)), dim3(256), 0, s, sums, ws.chunks, N, db);
+            if (vec) hipLaunchKernelGGL((slope_kernel<T, true>), grid, dim3(256), 0, s, dy, ldd, slope, dz, db ? sums : nullptr, M, N, act);
+            else hipLaunchKernelGGL((slope_kernel<T, false>), grid, dim3(256), 0, s, dy, ldd, slope, dz, db ? sums : nullptr, M, N, act);
+            if (db) hipLaunchKernelGGL(colsum_join_kernel<T>, dim3((unsigned)((N + 63) / 64)), dim3(64 * JOIN_WAVES), 0, s, sums, ws.chunks, N, db);
         });
     }
     const void* g = act != ACT_NONE ? dz : dy;

@@ -346,6 +346,9 @@ def _rows(t: torch.Tensor):
     return t, (t.stride(0) if rows > 1 else width)
 
 
+_SLOPE = (torch.float32, torch.int16, torch.int16)       # by DTYPES code
+
+
 @functools.lru_cache(maxsize=4096)
 def _linear_residual_bytes(M: int, N: int, K: int, dt: int, act: int = -1) -> int:
     lib = _lib.load()
@@ -354,10 +357,10 @@ def _linear_residual_bytes(M: int, N: int, K: int, dt: int, act: int = -1) -> in
 
 @on_data_device
 def linear_residual(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
-                    act: int = _lib.ACT_NONE, keep_pre: bool = False):
+                    act: int = _lib.ACT_NONE, keep_slope: bool = False):
     """``act(x w^T + bias) + residual`` in the tensors' own type (fp32, bf16 or fp16, all the same; fp32 sums, one rounding): x (..., K),
-    w (N, K), bias (N,), residual (..., N).  ``act``: ACT_NONE .. ACT_TANH.  ``keep_pre`` also returns the value before the activation, which
-    ``linear_residual_bwd`` needs.  Rows of x, w and residual may be strided (adjacent values in a row)."""
+    w (N, K), bias (N,), residual (..., N).  ``act``: ACT_NONE .. ACT_TANH.  ``keep_slope`` also returns the activation's slope, which
+    ``linear_residual_bwd`` needs: fp32 for fp32 tensors, 16-bit codes (see adx.h) in an int16 tensor otherwise.  Rows of x, w and residual may be strided (adjacent values in a row)."""
     dtype = x.dtype
     dt = DTYPES.get(dtype)
     if dt is None or w.dtype != dtype or (bias is not None and bias.dtype != dtype) or (residual is not None and residual.dtype != dtype):
@@ -372,7 +375,7 @@ def linear_residual(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tenso
         raise ValueError("linear_residual: bias (N,) and residual of the output's shape")
     stream = stream_on(device_of("linear_residual", x, w, bias, residual))
     y = x.new_empty(out_shape)
-    pre = x.new_empty(out_shape) if keep_pre else None
+    slope = x.new_empty(out_shape, dtype=_SLOPE[dt]) if keep_slope else None
     x2, ldx = _rows(x)
     M = x2.shape[0]
     if M:
@@ -382,28 +385,30 @@ def linear_residual(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tenso
         need = _linear_residual_bytes(M, N, K, dt)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         check(_lib.load().adx_op_linear_residual(x2.data_ptr(), ldx, w2.data_ptr(), ldw, None if b is None else b.data_ptr(),
-                                                 None if r2 is None else r2.data_ptr(), ldr, None if pre is None else pre.data_ptr(), y.data_ptr(), N,
+                                                 None if r2 is None else r2.data_ptr(), ldr, None if slope is None else slope.data_ptr(), y.data_ptr(), N,
                                                  M, N, K, act, dt, None if ws is None else ws.data_ptr(), need, stream), "linear_residual")
-    return (y, pre) if keep_pre else y
+    return (y, slope) if keep_slope else y
 
 
 @on_data_device
-def linear_residual_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pre: Optional[torch.Tensor] = None, act: int = _lib.ACT_NONE,
+def linear_residual_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, slope: Optional[torch.Tensor] = None, act: int = _lib.ACT_NONE,
                         need_dx: bool = True, need_dw: bool = True, need_db: bool = True):
-    """(dx, dw, db) of ``linear_residual`` from the gradient of its output, its operands and (unless act is ACT_NONE) the value before
-    the activation; None for those not asked for.  The gradient of the residual is dy."""
+    """(dx, dw, db) of ``linear_residual`` from the gradient of its output, its operands and (unless act is ACT_NONE) the slope that
+    the forward kept; None for those not asked for.  The gradient of the residual is dy."""
     dtype = dy.dtype
     dt = DTYPES.get(dtype)
-    if dt is None or x.dtype != dtype or w.dtype != dtype or (pre is not None and pre.dtype != dtype):
-        raise ValueError("linear_residual_bwd: dy, x, w and pre are fp32, bf16 or fp16, all the same")
+    if dt is None or x.dtype != dtype or w.dtype != dtype:
+        raise ValueError("linear_residual_bwd: dy, x and w are fp32, bf16 or fp16, all the same")
+    if slope is not None and slope.dtype != _SLOPE[dt]:
+        raise ValueError("linear_residual_bwd: slope is what linear_residual returned with keep_slope")
     if w.dim() != 2 or x.dim() < 1:
-        raise ValueError("linear_residual_bwd: x (..., K), w (N, K), dy and pre (..., N)")
+        raise ValueError("linear_residual_bwd: x (..., K), w (N, K), dy and slope (..., N)")
     N, K = w.shape
-    if x.shape[-1] != K or dy.shape != (*x.shape[:-1], N) or (pre is not None and pre.shape != dy.shape):
-        raise ValueError("linear_residual_bwd: x (..., K), w (N, K), dy and pre (..., N)")
-    if act != _lib.ACT_NONE and pre is None:
-        raise ValueError("linear_residual_bwd: the activation's gradient needs pre (linear_residual with keep_pre)")
-    stream = stream_on(device_of("linear_residual_bwd", dy, x, w, pre))
+    if x.shape[-1] != K or dy.shape != (*x.shape[:-1], N) or (slope is not None and slope.shape != dy.shape):
+        raise ValueError("linear_residual_bwd: x (..., K), w (N, K), dy and slope (..., N)")
+    if act != _lib.ACT_NONE and slope is None:
+        raise ValueError("linear_residual_bwd: the activation's gradient needs slope (linear_residual with keep_slope)")
+    stream = stream_on(device_of("linear_residual_bwd", dy, x, w, slope))
     g, ldd = _rows(dy)
     M = g.shape[0]
     dx = x.new_empty(x.shape) if need_dx else None
@@ -416,7 +421,7 @@ def linear_residual_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pre:
     elif need_dx or need_dw or need_db:
         x2, ldx = _rows(x)
         w2, ldw = _rows(w)
-        z = None if pre is None else pre.contiguous()
+        z = None if slope is None else slope.contiguous()
         need = _linear_residual_bytes(M, N, K, dt, act)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device)
         check(_lib.load().adx_op_linear_residual_bwd(g.data_ptr(), ldd, x2.data_ptr(), ldx, w2.data_ptr(), ldw, None if z is None else z.data_ptr(),

@@ -863,14 +863,14 @@ class _LinearResidual(torch.autograd.Function):
     def forward(ctx, x, w, bias, residual, act_code):
         need = ctx.needs_input_grad
         grad = need[0] or need[1] or need[2]
-        pre = None
+        slope = None
         if grad and act_code != _lib.ACT_NONE:
-            y, pre = ops.linear_residual(x, w, bias, residual, act_code, True)
+            y, slope = ops.linear_residual(x, w, bias, residual, act_code, True)
         else:
             y = ops.linear_residual(x, w, bias, residual, act_code)
         ctx.act_code = act_code
         if grad:
-            ctx.save_for_backward(x, w, pre)
+            ctx.save_for_backward(x, w, slope)
         return y
 
     @staticmethod
@@ -879,12 +879,13 @@ class _LinearResidual(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx = dw = db = None
         if need[0] or need[1] or need[2]:
-            x, w, pre = ctx.saved_tensors
-            dx, dw, db = ops.linear_residual_bwd(dy, x, w, pre, ctx.act_code, need[0], need[1], need[2])
+            x, w, slope = ctx.saved_tensors
+            dx, dw, db = ops.linear_residual_bwd(dy, x, w, slope, ctx.act_code, need[0], need[1], need[2])
         return dx, dw, db, dy if need[3] else None, None
 
 
 def linear_residual(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
                     act: int = _lib.ACT_NONE) -> torch.Tensor:
-    """``ops.linear_residual`` with gradients for x, w, bias and residual.  The value before the activation is kept in the tensors' type."""
+    """``ops.linear_residual`` with gradients for x, w, bias and residual.  For the backward it keeps x, w and the
+    activation's slope (in 16 bits where the tensors have 16)."""
     return _LinearResidual.apply(x, w, bias, residual, act)

@@ -306,18 +306,19 @@ int adx_op_rope(const void* q, void* q_out, int heads_q, const void* k, void* k_
                 const int64_t* positions, int64_t pos_stride_b, int64_t pos_stride_s, int64_t pos0, const double* inv_freq, float amplitude,
                 int B, int S, int dh, int rotary_dim, int interleaved, int inverse, int dtype, void* stream);
 /* y[M][N] = act(x[M][K] w[N][K]^T + bias[N]) + res[M][N]; bias, res nullable; all tensors of one element type; row strides (elements)
- * ldx, ldw, ldr, ldy >= N, adjacent values in a row (ldr = 0: one row for all).  pre (nullable, [M][N] contiguous) receives the value
- * before the activation, which the gradient needs for act != ADX_ACT_NONE.  act: ADX_ACT_NONE .. ADX_ACT_TANH.  y and pre overlap no input,
- * except that y may be res itself (same pointer and stride).  M = 0 does nothing.
+ * ldx, ldw, ldr, ldy >= N, adjacent values in a row (ldr = 0: one row for all).  act: ADX_ACT_NONE .. ADX_ACT_TANH.  slope (nullable,
+ * [M][N] contiguous) receives what the gradient needs for act != ADX_ACT_NONE, act' of the sum: fp32 values for fp32 tensors; for 16-bit
+ * tensors uint16 codes q of (q - 8192) / 32768 (65535: NaN), or for ADX_ACT_RELU and ADX_ACT_LEAKY 1 where the sum is positive, else 0.
+ * y and slope overlap no input, except that y may be res itself (same pointer and stride).  M = 0 does nothing.
  * workspace: adx_linear_residual_ws_bytes(M, N, K, dtype) bytes, 16-byte aligned (0: may be NULL), the call's own until it has run. */
 size_t adx_linear_residual_ws_bytes(int64_t M, int N, int K, int dtype);
-int adx_op_linear_residual(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldr, void* pre,
+int adx_op_linear_residual(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldr, void* slope,
                            void* y, int64_t ldy, int64_t M, int N, int K, int act, int dtype, void* workspace, size_t workspace_bytes, void* stream);
-/* Its gradients, any of them NULL where not wanted: with dz = dy act'(pre), dx[M][K] = dz w, dw[N][K] = dz^T x, db[N] = column sums of
- * dz (the residual's gradient is dy itself).  pre may be NULL for ADX_ACT_NONE.  dz is rounded to the element type as the operand of the two
+/* Its gradients, any of them NULL where not wanted: with dz = dy slope, dx[M][K] = dz w, dw[N][K] = dz^T x, db[N] = column sums of
+ * dz (the residual's gradient is dy itself).  slope may be NULL for ADX_ACT_NONE.  dz is rounded to the element type as the operand of the two
  * products; db sums the unrounded values.  Sums over rows are joined in a fixed order (no atomics): bit-identical re-runs. */
 size_t adx_linear_residual_bwd_ws_bytes(int64_t M, int N, int K, int act, int dtype);
-int adx_op_linear_residual_bwd(const void* dy, int64_t ldd, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* pre, void* dx,
+int adx_op_linear_residual_bwd(const void* dy, int64_t ldd, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* slope, void* dx,
                                void* dw, void* db, int64_t M, int N, int K, int act, int dtype, void* workspace, size_t workspace_bytes,
                                void* stream);
 /* adx_op_moe_block for a few tokens (1 <= T <= 64; d, inter multiples of 32): the same expert layer in two kernels (three where the

@@ -60,10 +60,10 @@ def test_linear_residual_abi_refusals():
 def test_linear_residual_bwd_abi_refusals():
     lib = _lib.load()
 
-    def call(dy=FAKE, x=FAKE, w=FAKE, pre=FAKE, dx=FAKE, dw=FAKE, db=FAKE, M=100, N=64, K=64, act=2, dt=BF16, ws=FAKE, n=1 << 40):
-        return lib.adx_op_linear_residual_bwd(dy, N, x, K, w, K, pre, dx, dw, db, M, N, K, act, dt, ws, n, None)
+    def call(dy=FAKE, x=FAKE, w=FAKE, slope=FAKE, dx=FAKE, dw=FAKE, db=FAKE, M=100, N=64, K=64, act=2, dt=BF16, ws=FAKE, n=1 << 40):
+        return lib.adx_op_linear_residual_bwd(dy, N, x, K, w, K, slope, dx, dw, db, M, N, K, act, dt, ws, n, None)
 
-    for bad in (dict(dy=None), dict(x=None), dict(w=None), dict(pre=None)):
+    for bad in (dict(dy=None), dict(x=None), dict(w=None), dict(slope=None)):
         refused(call(**bad), b"null pointer")
     refused(call(dt=-1), b"element type")
     refused(call(act=9), b"activation")
@@ -116,7 +116,9 @@ def test_python_refusals():
     with pytest.raises(_lib.AdxError, match="device memory"):
         train.linear_residual(x.requires_grad_(), wt)
     with pytest.raises(ValueError):
-        ops.linear_residual_bwd(torch.zeros(5, 8), x, wt, None, act=2)                       # no value before the activation
+        ops.linear_residual_bwd(torch.zeros(5, 8), x, wt, None, act=2)                       # no slope
+    with pytest.raises(ValueError):
+        ops.linear_residual_bwd(torch.zeros(5, 8), x, wt, torch.zeros(5, 8, dtype=torch.int16), act=2)        # a slope of another type
     with pytest.raises(ValueError):
         ops.linear_residual_bwd(torch.zeros(5, 7), x, wt)
     t, r, w13, w2 = torch.zeros(4, 32), torch.zeros(8, 32), torch.zeros(8, 128, 32), torch.zeros(8, 32, 64)
