@@ -18,25 +18,32 @@ constexpr int ACT_TANH_ = 6;
 __device__ __align__(16) unsigned char zero_chunk[16];            // what copies past the end of the summed axis read
 
 // ------------------------------------------------------------------------------------------------------------- activations
-// erfc(u) / 2 for u >= 0, times exp(u^2): a polynomial in 1 / (1 + u / 2) (the Chebyshev fit of the textbooks, fractional error 1.2e-7:
-// two fp32 roundings, also in the tail, where 1 - erf has none left).  A quarter of the instructions of erff.
-__device__ __forceinline__ float half_erfc_scaled_log(float t) {
-    float p = 0.17087277f;
-    p = p * t - 0.82215223f; p = p * t + 1.48851587f; p = p * t - 1.13520398f; p = p * t + 0.27886807f; p = p * t - 0.18628806f;
-    p = p * t + 0.09678418f; p = p * t + 0.37409196f; p = p * t + 1.00002368f;
-    return p * t - 1.26551223f;
-}
-// Phi(-|z|), the smaller tail of the normal distribution
-__device__ __forceinline__ float normal_tail(float z) {
-    const float u = fabsf(z) * 0.70710678118654752f, t = rcp_fast(1.f + 0.5f * u);
-    return 0.5f * t * exp2_fast((half_erfc_scaled_log(t) - u * u) * 1.44269504088896341f);
+// Phi(-|z|), the smaller tail of the normal distribution, and e = exp(-z^2 / 2).  fp32 tensors: the textbooks' Chebyshev fit of erfc
+// (fractional error 1.2e-7, also in the tail, where 1 - erf has none left).  16-bit tensors: e times a polynomial in t = 1 / (1 + 0.44 |z| /
+// sqrt 2), fitted to Phi(-|z|) / (t e) for |z| <= 13 (5e-7 with its fp32 rounding), which shares its exponential with the slope: the
+// activation of a 256 x 256 tile is as long as a quarter of its products at k = 1024.
+template <typename T> __device__ __forceinline__ float normal_tail(float z, float& e) {
+    e = exp2_fast(-0.72134752044448170f * z * z);
+    if constexpr (sizeof(T) == 2) {
+        const float t = rcp_fast(1.f + 0.3111269772052765f * fabsf(z));
+        float p = 0.035492222756147385f;
+        p = p * t - 0.13845060765743256f; p = p * t + 0.14739154279232025f; p = p * t - 0.009160763584077358f; p = p * t + 0.10738220810890198f;
+        p = p * t + 0.10882654786109924f; p = p * t + 0.12440642714500427f; p = p * t + 0.12411251664161682f;
+        return p * t * e;
+    } else {
+        const float u = fabsf(z) * 0.70710678118654752f, t = rcp_fast(1.f + 0.5f * u);
+        float p = 0.17087277f;
+        p = p * t - 0.82215223f; p = p * t + 1.48851587f; p = p * t - 1.13520398f; p = p * t + 0.27886807f; p = p * t - 0.18628806f;
+        p = p * t + 0.09678418f; p = p * t + 0.37409196f; p = p * t + 1.00002368f; p = p * t - 1.26551223f;
+        return 0.5f * t * exp2_fast((p - u * u) * 1.44269504088896341f);
+    }
 }
 __device__ __forceinline__ float sigmoid_fast(float z) { return rcp_fast(1.f + exp2_fast(-1.44269504088896341f * z)); }
 // z + 0.044715 z^3 scaled so that its sigmoid is (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2
 __device__ __forceinline__ float gelu_tanh_arg(float z) { return 1.59576912160573071f * z * (1.f + 0.044715f * z * z); }
 
 // act(z) in place and, with SLOPE, act'(z) from the same exponentials
-template <int V, bool SLOPE> __device__ __forceinline__ void apply_act(float (&v)[V], float (&d)[V], int act) {
+template <typename T, int V, bool SLOPE> __device__ __forceinline__ void apply_act(float (&v)[V], float (&d)[V], int act) {
     switch (act) {                                                 // uniform: one branch for all values
         case ACT_RELU:
 #pragma unroll
@@ -57,8 +64,9 @@ template <int V, bool SLOPE> __device__ __forceinline__ void apply_act(float (&v
         case ACT_GELU_ERF:
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float q = normal_tail(v[e]), p = v[e] > 0.f ? 1.f - q : q;
-                if (SLOPE) d[e] = p + v[e] * 0.39894228040143268f * exp2_fast(-0.72134752044448170f * v[e] * v[e]);
+                float g;
+                const float q = normal_tail<T>(v[e], g), p = v[e] > 0.f ? 1.f - q : q;
+                if (SLOPE) d[e] = p + v[e] * 0.39894228040143268f * g;
                 v[e] *= p;
             }
             break;
@@ -82,22 +90,16 @@ template <int V, bool SLOPE> __device__ __forceinline__ void apply_act(float (&v
 
 // What the forward keeps for the gradient is the activation's slope, not its argument: the backward needs no exponentials, and in 16
 // bits a slope (-0.13 .. 1.13) fits to 2^-16 as a fixed-point number, where an argument rounded to bf16 moves the gradient as much
-// as the rounding of dz does.  fp32 tensors keep it as it is.  Codes: (q - 8192) / 32768, 65535 for NaN, the piecewise activations 1 where
-// the argument is positive.
+// as the rounding of dz does.  fp32 tensors keep it as it is.  Codes: q stands for (q - 8192) / 32768, 0 for NaN (what the conversion of
+// one gives), and LeakyReLU's two for 1 and 0.01 themselves.
 template <typename T> struct Slope { typedef unsigned short type; };
 template <> struct Slope<float> { typedef float type; };
-__device__ __forceinline__ float slope_code(float d, int act, float) { return d; }
-__device__ __forceinline__ unsigned short slope_code(float d, int act, unsigned short) {
-    if (d != d) return 65535;
-    if (act == ACT_RELU || act == ACT_LEAKY) return d == 1.f;
-    return (unsigned short)(int)rintf(d * 32768.f + 8192.f);
-}
+__device__ __forceinline__ void set_code(float d, float& q) { q = d; }
+__device__ __forceinline__ void set_code(float d, unsigned short& q) { q = (unsigned short)(unsigned)(d * 32768.f + 8192.5f); }
 __device__ __forceinline__ float slope_value(float q, int act) { return q; }
 __device__ __forceinline__ float slope_value(unsigned short q, int act) {
-    if (q == 65535) return __builtin_nanf("");
-    if (act == ACT_RELU) return (float)q;
-    if (act == ACT_LEAKY) return q ? 1.f : 0.01f;
-    return (float)((int)q - 8192) * (1.f / 32768.f);
+    const float d = act == ACT_LEAKY ? (q > 16384 ? 1.f : 0.01f) : (float)((int)q - 8192) * (1.f / 32768.f);
+    return q ? d : __builtin_nanf("");
 }
 
 // ------------------------------------------------------------------------------------------------------------- the problem
@@ -115,13 +117,16 @@ struct ProductArgs {
     int tiles_m, tiles_n;
 };
 
-// V consecutive columns of one row: bias, activation, residual, one rounding, store
+// V consecutive columns of one row: bias, activation, residual, one rounding, store.  `r`: the residual's values (vec)
 template <typename T, int V>
-__device__ __forceinline__ void finish(const ProductArgs& a, int64_t m, int n, float (&v)[V], bool vec) {
+__device__ __forceinline__ Pack<T, V> residual_at(const ProductArgs& a, int64_t m, int n) {
+    return *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.res) + m * a.ldr + n);
+}
+template <typename T, int V>
+__device__ __forceinline__ void finish(const ProductArgs& a, int64_t m, int n, float (&v)[V], bool vec, const Pack<T, V>& r) {
     typedef typename Slope<T>::type S;
     T* y = static_cast<T*>(a.y) + m * a.ldy + n;
     const T* bias = static_cast<const T*>(a.bias);
-    const T* res = static_cast<const T*>(a.res) + (a.res ? m * a.ldr + n : 0);
     S* slope = static_cast<S*>(a.slope) + (a.slope ? m * a.N + n : 0);
     typedef Pack<T, V> P;
     float d[V];
@@ -132,14 +137,13 @@ __device__ __forceinline__ void finish(const ProductArgs& a, int64_t m, int n, f
             for (int e = 0; e < V; ++e) v[e] += (float)b.v[e];
         }
         if (a.slope) {
-            apply_act<V, true>(v, d, a.act);
+            apply_act<T, V, true>(v, d, a.act);
             Pack<S, V> q;
 #pragma unroll
-            for (int e = 0; e < V; ++e) q.v[e] = slope_code(d[e], a.act, S());
+            for (int e = 0; e < V; ++e) set_code(d[e], q.v[e]);
             *reinterpret_cast<Pack<S, V>*>(slope) = q;
-        } else apply_act<V, false>(v, d, a.act);
+        } else apply_act<T, V, false>(v, d, a.act);
         if (a.res) {
-            const P r = *reinterpret_cast<const P*>(res);
 #pragma unroll
             for (int e = 0; e < V; ++e) v[e] += (float)r.v[e];
         }
@@ -148,17 +152,24 @@ __device__ __forceinline__ void finish(const ProductArgs& a, int64_t m, int n, f
         for (int e = 0; e < V; ++e) o.v[e] = (T)v[e];
         *reinterpret_cast<P*>(y) = o;
     } else {
+        const T* res = static_cast<const T*>(a.res) + (a.res ? m * a.ldr + n : 0);
 #pragma unroll
         for (int e = 0; e < V; ++e) if (bias && n + e < a.N) v[e] += (float)bias[n + e];
-        apply_act<V, true>(v, d, a.act);
+        apply_act<T, V, true>(v, d, a.act);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             if (n + e >= a.N) break;
-            if (a.slope) slope[e] = slope_code(d[e], a.act, S());
+            if (a.slope) set_code(d[e], slope[e]);
             if (a.res) v[e] += (float)res[e];
             y[e] = (T)v[e];
         }
     }
+}
+template <typename T, int V>
+__device__ __forceinline__ void finish(const ProductArgs& a, int64_t m, int n, float (&v)[V], bool vec) {
+    Pack<T, V> r{};
+    if (vec && a.res) r = residual_at<T, V>(a, m, n);
+    finish<T, V>(a, m, n, v, vec, r);
 }
 
 // ------------------------------------------------------------------------------------------------------------- large tiles
@@ -255,6 +266,15 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, f32x16_t (&acc)
     constexpr int NW = FJ * 32, EP_LD = NW + 4, V = 16 / sizeof(T), LPR = NW / V, RPI = 64 / LPR;   // lanes of a row, rows of one pass
     float* patch = reinterpret_cast<float*>(smem) + wave * 32 * EP_LD;
     const int n = n_wave + (lane % LPR) * V;
+    // the residual is read a pass ahead: sixteen passes of 256 x 256 tiles would wait for it one after the other
+    const bool ahead = a.res && a.vec && a.splits <= 1;
+    const int64_t m_last = a.M - 1;
+    auto residual = [&](int row) {                             // row of the wave's tile; past the end of the tensor: the last row
+        const int64_t m = m_wave + row;
+        return residual_at<T, V>(a, m < m_last ? m : m_last, n < a.N ? n : 0);
+    };
+    Pack<T, V> r_next{};
+    if (ahead) r_next = residual(lane / LPR);
 #pragma unroll
     for (int i = 0; i < FI; ++i) {
         __builtin_amdgcn_wave_barrier();
@@ -270,6 +290,8 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, f32x16_t (&acc)
         for (int p = 0; p < 32 / RPI; ++p) {
             const int r = p * RPI + lane / LPR;
             const int64_t m = m_wave + i * 32 + r;
+            const Pack<T, V> rv = r_next;
+            if (ahead) r_next = residual(i * 32 + r + RPI);
             float v[V];
 #pragma unroll
             for (int e = 0; e < V; e += 4) {
@@ -286,7 +308,7 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, f32x16_t (&acc)
 #pragma unroll
                         for (int e = 0; e < V; ++e) if (n + e < a.N) o[e] = v[e];
                     }
-                } else finish<T, V>(a, m, n, v, a.vec);
+                } else finish<T, V>(a, m, n, v, a.vec, rv);
             }
         }
         wait_lds();
@@ -587,7 +609,7 @@ __global__ __launch_bounds__(64 * NWAVES) void product_few_kernel(const ProductA
 constexpr int SLOPE_ROWS = 64;
 
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void slope_kernel(const void* dy_, int64_t ldd, const void* slope_, void* dz_, float* part, int64_t M, int N, int act) {
+__global__ __launch_bounds__(256) void slope_kernel(const void* dy_, int64_t ldd, const void* slope_, void* dz_, float* part, void* db, int64_t M, int N, int act) {
     constexpr int V = VEC ? 16 / sizeof(T) : 1;
     typedef typename Slope<T>::type S;
     __shared__ float sums[4][64 * V];
@@ -624,7 +646,10 @@ __global__ __launch_bounds__(256) void slope_kernel(const void* dy_, int64_t ldd
     __syncthreads();
     for (int i = threadIdx.x; i < 64 * V; i += 256) {
         const int col = blockIdx.x * 64 * V + i;
-        if (col < N) part[(int64_t)blockIdx.y * N + col] = (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
+        if (col >= N) continue;
+        const float s = (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
+        if (db) static_cast<T*>(db)[col] = (T)s;                // all rows in one chunk
+        else part[(int64_t)blockIdx.y * N + col] = s;
     }
 }
 
@@ -651,17 +676,21 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void colsum_join_kernel(const floa
 // ------------------------------------------------------------------------------------------------------------- host
 struct Plan { int tile; int splits; int64_t k_split; size_t part_bytes; };       // tile: 0 few rows, else its edge
 
+// Few rows: the streaming kernel.  Else the largest tile that still gives most CUs one (256: one workgroup a CU, 200 of 256 CUs; 128 and
+// 64: several a CU hide each other's waits).  Tiles of 64 split the summed axis up to four workgroups a CU as long as each keeps 20
+// steps of 128 bytes (8 where the tiles alone leave half of the card idle): 1024 x 1024 x 4096 bf16 26 us in one part, 23 in three; the join
+// costs 5 us, so that 1037 x 1024 x 1024 takes 11 us in one part and 15 in two.
 Plan plan_product(int64_t M, int N, int64_t K, int dt, bool acol, bool bcol) {
     Plan p{0, 1, K, 0};
     if (!acol && !bcol && M <= 64) return p;
     const int64_t ke = 128 / dtype_bytes(dt);                 // K step of the tiles
     auto tiles = [&](int64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
-    p.tile = tiles(256) >= 200 ? 256 : tiles(128) >= 200 ? 128 : 64;
+    p.tile = tiles(256) >= 200 ? 256 : tiles(128) >= 400 ? 128 : 64;
     const int64_t steps = (K + ke - 1) / ke;
     p.k_split = steps * ke;
-    if (p.tile == 64 && tiles(64) < 256) {
-        int64_t want = 512 / tiles(64);
-        const int64_t most = steps / 8;
+    if (p.tile == 64) {
+        const int64_t n = tiles(64), most = steps / (n < 128 ? 8 : 20);
+        int64_t want = 1024 / n;
         want = want < most ? want : most;
         if (want > 1) {
             const int64_t per = (steps + want - 1) / want;
@@ -677,8 +706,10 @@ template <typename T, bool ACOL, bool BCOL, int EDGE>
 void launch_tile(const ProductArgs& a, hipStream_t s) {
     const int n_tiles = a.tiles_m * a.tiles_n;
     const dim3 grid((unsigned)((n_tiles + 7) / 8 * 8), (unsigned)a.splits);
-    constexpr int WN = EDGE == 256 ? 4 : 2;
-    hipLaunchKernelGGL((product_kernel<T, ACOL, BCOL, EDGE, EDGE, 2, WN, 128, 2>), grid, dim3(128 * WN), 0, s, a);
+    // 256: 238 us for 8192 x 4096 x 4096 bf16 with steps of 128 bytes in two slots, 250 - 270 with 64 in four, 279 with four waves of 128 x 128;
+    // 64: 26 us for 1024 x 1024 x 4096 with 64 in four, 34 with 128 in two
+    constexpr int WN = EDGE == 256 ? 4 : 2, KB = EDGE == 64 ? 64 : 128, R = EDGE == 64 ? 4 : 2;
+    hipLaunchKernelGGL((product_kernel<T, ACOL, BCOL, EDGE, EDGE, 2, WN, KB, R>), grid, dim3(128 * WN), 0, s, a);
 }
 
 template <typename T, int MT, int NT, int NWAVES>
@@ -810,9 +841,9 @@ ADX_API int adx_op_linear_residual_bwd(const void* dy, int64_t ldd, const void* 
             typedef decltype(t) T;
             const int cols = vec ? 64 * V : 64;
             const dim3 grid((unsigned)((N + cols - 1) / cols), (unsigned)ws.chunks);
-            if (vec) hipLaunchKernelGGL((slope_kernel<T, true>), grid, dim3(256), 0, s, dy, ldd, slope, dz, db ? sums : nullptr, M, N, act);
-            else hipLaunchKernelGGL((slope_kernel<T, false>), grid, dim3(256), 0, s, dy, ldd, slope, dz, db ? sums : nullptr, M, N, act);
-            if (db) hipLaunchKernelGGL(colsum_join_kernel<T>, dim3((unsigned)((N + 63) / 64)), dim3(64 * JOIN_WAVES), 0, s, sums, ws.chunks, N, db);
+            if (vec) hipLaunchKernelGGL((slope_kernel<T, true>), grid, dim3(256), 0, s, dy, ldd, slope, dz, db ? sums : nullptr, ws.chunks == 1 ? db : nullptr, M, N, act);
+            else hipLaunchKernelGGL((slope_kernel<T, false>), grid, dim3(256), 0, s, dy, ldd, slope, dz, db ? sums : nullptr, ws.chunks == 1 ? db : nullptr, M, N, act);
+            if (db && ws.chunks > 1) hipLaunchKernelGGL(colsum_join_kernel<T>, dim3((unsigned)((N + 63) / 64)), dim3(64 * JOIN_WAVES), 0, s, sums, ws.chunks, N, db);
         });
     }
     const void* g = act != ACT_NONE ? dz : dy;

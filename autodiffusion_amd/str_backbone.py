@@ -184,11 +184,13 @@ class KVCache:
 
 class MixtralModel(nn.Module):
     """Parameter holder + device forward of the sparse mixture-of-experts decoder on input embeddings (causal mask, positions
-    0, 1, 2, ...).  ``precision``: operand type of the products ("fp32" | "bf16" | "bf16x3"); the router computes in fp32."""
+    0, 1, 2, ...).  ``precision``: operand type of the products ("fp32" | "bf16" | "bf16x3"); the router computes in fp32.
+    ``few_token_experts``: passes of at most 64 tokens (the key points of a batch) run their expert layers through ``moe_few`` -- two
+    kernels instead of seven, tokens and hidden values not rounded to the weights' type, so that "bf16" results differ from the default's."""
 
     def __init__(self, hidden_size: int, intermediate_size: int, num_hidden_layers: int, num_attention_heads: int, num_key_value_heads: int = 8,
                  num_local_experts: int = 8, num_experts_per_tok: int = 2, rms_norm_eps: float = 1e-5, rope_theta: float = 1e6,
-                 vocab_size: int = 32000, sliding_window: Optional[int] = 4096, precision: str = "fp32"):
+                 vocab_size: int = 32000, sliding_window: Optional[int] = 4096, precision: str = "fp32", few_token_experts: bool = False):
         super().__init__()
         if hidden_size % num_attention_heads or num_attention_heads % num_key_value_heads or (hidden_size // num_attention_heads) % 2:
             raise ValueError("MixtralModel: hidden size divisible by the head count, head count by the key / value head count, even head width")
@@ -201,7 +203,7 @@ class MixtralModel(nn.Module):
         self.norm = _RMS(hidden_size)
         self.d, self.inter, self.n_head, self.n_kv = hidden_size, intermediate_size, num_attention_heads, num_key_value_heads
         self.n_experts, self.top_k, self.eps, self.theta = num_local_experts, num_experts_per_tok, float(rms_norm_eps), float(rope_theta)
-        self.sliding_window, self.precision = sliding_window, precision
+        self.sliding_window, self.precision, self.few_token_experts = sliding_window, precision, bool(few_token_experts)
         self._prepared: Dict[str, torch.Tensor] = {}
         self._stamp = None
         self._tables = None
@@ -277,8 +279,10 @@ class MixtralModel(nn.Module):
             att = ops.attention(q, K, V, H, mask_off=past, precision=self.precision)
             x = _add(x, lin(att, f"{i}.o_proj", d))
             n2 = rmsnorm(x, layer.post_attention_layernorm.weight, self.eps)
-            r = moe_block(n2.reshape(B * n, d), x.reshape(B * n, d), W[f"{i}.gate"], W[f"{i}.w13"], W[f"{i}.w2"], self.inter, self.n_experts,
-                          self.top_k, self.precision, self._workspace(B * n, x.device), return_routing)
+            few = self.few_token_experts and B * n <= 64
+            r = (moe_few if few else moe_block)(n2.reshape(B * n, d), x.reshape(B * n, d), W[f"{i}.gate"], W[f"{i}.w13"], W[f"{i}.w2"], self.inter,
+                                                self.n_experts, self.top_k, self.precision, None if few else self._workspace(B * n, x.device),
+                                                return_routing)
             if return_routing:
                 r, idx, wts = r
                 routing.append((idx, wts))
@@ -332,7 +336,7 @@ def str_config(model_name: str = "mixtral-small", **kw) -> SimpleNamespace:
                 x_random_walk=0.0, y_random_walk=0.0, arf_x_random_walk=0.0, arf_y_random_walk=0.0, predict_yaw=True, loss_fn="mse",
                 trajectory_decoder_type="mlp", traj_dropout=0.0, kp_dropout=0.0, mean_circular_loss=True, trajectory_prediction_mode="all_frames",
                 pred_key_points_only=False, trajectory_loss_rescale=1.0, reverse_traj_index_order=False, num_key_value_heads=8,
-                num_local_experts=8, num_experts_per_tok=2, rms_norm_eps=1e-5, rope_theta=1e6, sliding_window=4096)
+                num_local_experts=8, num_experts_per_tok=2, rms_norm_eps=1e-5, rope_theta=1e6, sliding_window=4096, few_token_experts=False)
     base.update(mixtral_sizes(model_name))
     base.update(kw)
     return SimpleNamespace(**base)
@@ -360,7 +364,8 @@ class STR_Mixtral(nn.Module):
         self.transformer = MixtralModel(cfg.n_embd, cfg.n_inner, cfg.n_layer, cfg.n_head, getattr(cfg, "num_key_value_heads", 8),
                                         getattr(cfg, "num_local_experts", 8), getattr(cfg, "num_experts_per_tok", 2),
                                         getattr(cfg, "rms_norm_eps", 1e-5), getattr(cfg, "rope_theta", 1e6),
-                                        sliding_window=getattr(cfg, "sliding_window", 4096), precision=precision)
+                                        sliding_window=getattr(cfg, "sliding_window", 4096), precision=precision,
+                                        few_token_experts=getattr(cfg, "few_token_experts", False))
         if self.use_key_points != "no":
             if getattr(cfg, "kp_decoder_type", "mlp") != "mlp":
                 raise NotImplementedError("STR_Mixtral: only the MLP key-point head is built (kp_decoder_type='mlp')")

@@ -308,7 +308,7 @@ int adx_op_rope(const void* q, void* q_out, int heads_q, const void* k, void* k_
 /* y[M][N] = act(x[M][K] w[N][K]^T + bias[N]) + res[M][N]; bias, res nullable; all tensors of one element type; row strides (elements)
  * ldx, ldw, ldr, ldy >= N, adjacent values in a row (ldr = 0: one row for all).  act: ADX_ACT_NONE .. ADX_ACT_TANH.  slope (nullable,
  * [M][N] contiguous) receives what the gradient needs for act != ADX_ACT_NONE, act' of the sum: fp32 values for fp32 tensors; for 16-bit
- * tensors uint16 codes q of (q - 8192) / 32768 (65535: NaN), or for ADX_ACT_RELU and ADX_ACT_LEAKY 1 where the sum is positive, else 0.
+ * tensors uint16 codes q of (q - 8192) / 32768 (0: NaN; LeakyReLU's 8520 stands for 0.01 itself).
  * y and slope overlap no input, except that y may be res itself (same pointer and stride).  M = 0 does nothing.
  * workspace: adx_linear_residual_ws_bytes(M, N, K, dtype) bytes, 16-byte aligned (0: may be NULL), the call's own until it has run. */
 size_t adx_linear_residual_ws_bytes(int64_t M, int N, int K, int dtype);
