@@ -349,6 +349,14 @@ def _rows(t: torch.Tensor):
 _SLOPE = (torch.float32, torch.int16, torch.int16)       # by DTYPES code
 
 
+def _on_pieces(t: torch.Tensor, ld: int):
+    """(tensor, row stride) with rows that start on 16 bytes, if whole 16-byte pieces make up a row (else the library lays it out anew)."""
+    size, width = t.element_size(), t.shape[1]
+    if width * size % 16 == 0 and (ld * size % 16 or t.data_ptr() % 16):
+        t, ld = t.clone(memory_format=torch.contiguous_format), width
+    return t, ld
+
+
 @functools.lru_cache(maxsize=4096)
 def _linear_residual_bytes(M: int, N: int, K: int, dt: int, act: int = -1) -> int:
     lib = _lib.load()
@@ -380,6 +388,8 @@ def linear_residual(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tenso
     M = x2.shape[0]
     if M:
         w2, ldw = _rows(w)
+        if M > 64:                                       # fewer rows are read where they lie
+            (x2, ldx), (w2, ldw) = _on_pieces(x2, ldx), _on_pieces(w2, ldw)
         b = None if bias is None else bias.contiguous()
         r2, ldr = (None, 0) if residual is None else _rows(residual)
         need = _linear_residual_bytes(M, N, K, dt)
@@ -419,8 +429,7 @@ def linear_residual_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, slop
             if t is not None:
                 t.zero_()
     elif need_dx or need_dw or need_db:
-        x2, ldx = _rows(x)
-        w2, ldw = _rows(w)
+        (x2, ldx), (w2, ldw), (g, ldd) = _on_pieces(*_rows(x)), _on_pieces(*_rows(w)), _on_pieces(g, ldd)
         z = None if slope is None else slope.contiguous()
         need = _linear_residual_bytes(M, N, K, dt, act)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device)

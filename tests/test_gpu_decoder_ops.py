@@ -258,6 +258,8 @@ def test_linear_residual_bwd(dev, kind, M, N, K):
         assert all(torch.equal(a, b) for a, b in zip((dx, dw, db), again))
     slope, _ = slope_codes(z, "silu", kind)
     only = ops.linear_residual_bwd(dy, x, w, slope, act=5, need_dx=False, need_db=False)
+    bias_only = ops.linear_residual_bwd(dy, x, w, slope, act=5, need_dx=False, need_dw=False)
+    assert bias_only[0] is None and bias_only[1] is None and torch.equal(bias_only[2], ops.linear_residual_bwd(dy, x, w, slope, act=5)[2])
     assert only[0] is None and only[2] is None and torch.equal(only[1], ops.linear_residual_bwd(dy, x, w, slope, act=5)[1])
 
 
@@ -280,7 +282,8 @@ def test_linear_residual_gradient_of_rows_that_are_not_finite(dev):
 def test_linear_residual_bwd_large(dev):
     from autodiffusion_amd import ops
     g = torch.Generator().manual_seed(9)
-    for kind, M, N, K in (("bf16", 3000, 4104, 3600), ("fp32", 1037, 1020, 772), ("fp16", 8200, 264, 200)):
+    for kind, M, N, K in (("bf16", 3000, 4104, 3600), ("fp32", 1037, 1020, 772), ("fp16", 8200, 264, 200),
+                          ("bf16", 3186, 206, 4651), ("fp16", 2051, 2053, 2055), ("fp32", 900, 1021, 771), ("bf16", 700, 1203, 64)):
         x, w, dy = rand(g, M, K, kind=kind), rand(g, N, K, kind=kind, scale=K ** -0.5), rand(g, M, N, kind=kind)
         dx, dw, db = ops.linear_residual_bwd(dy, x, w)
         d, aw, ax = dy.double(), w.double().abs(), x.double().abs()
