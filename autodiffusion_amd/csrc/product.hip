@@ -18,25 +18,16 @@ constexpr int ACT_TANH_ = 6;
 __device__ __align__(16) unsigned char zero_chunk[16];            // what copies past the end of the summed axis read
 
 // ------------------------------------------------------------------------------------------------------------- activations
-// Phi(-|z|), the smaller tail of the normal distribution, and e = exp(-z^2 / 2).  fp32 tensors: the textbooks' Chebyshev fit of erfc
-// (fractional error 1.2e-7, also in the tail, where 1 - erf has none left).  16-bit tensors: e times a polynomial in t = 1 / (1 + 0.44 |z| /
-// sqrt 2), fitted to Phi(-|z|) / (t e) for |z| <= 13 (5e-7 with its fp32 rounding), which shares its exponential with the slope: the
-// activation of a 256 x 256 tile is as long as a quarter of its products at k = 1024.
-template <typename T> __device__ __forceinline__ float normal_tail(float z, float& e) {
+// Phi(-|z|), the smaller tail of the normal distribution, and e = exp(-z^2 / 2): e times a polynomial in t = 1 / (1 + 0.35 |z|), fitted to
+// Phi(-|z|) / (t e) for |z| <= 13 (relative error 3e-8, 3e-7 with the roundings in fp32; 1 - erf would have no digits left in the tail).  The
+// slope shares the exponential: the activation of a 256 x 256 tile is as long as a quarter of its products at k = 1024.
+__device__ __forceinline__ float normal_tail(float z, float& e) {
     e = exp2_fast(-0.72134752044448170f * z * z);
-    if constexpr (sizeof(T) == 2) {
-        const float t = rcp_fast(1.f + 0.3111269772052765f * fabsf(z));
-        float p = 0.035492222756147385f;
-        p = p * t - 0.13845060765743256f; p = p * t + 0.14739154279232025f; p = p * t - 0.009160763584077358f; p = p * t + 0.10738220810890198f;
-        p = p * t + 0.10882654786109924f; p = p * t + 0.12440642714500427f; p = p * t + 0.12411251664161682f;
-        return p * t * e;
-    } else {
-        const float u = fabsf(z) * 0.70710678118654752f, t = rcp_fast(1.f + 0.5f * u);
-        float p = 0.17087277f;
-        p = p * t - 0.82215223f; p = p * t + 1.48851587f; p = p * t - 1.13520398f; p = p * t + 0.27886807f; p = p * t - 0.18628806f;
-        p = p * t + 0.09678418f; p = p * t + 0.37409196f; p = p * t + 1.00002368f; p = p * t - 1.26551223f;
-        return 0.5f * t * exp2_fast((p - u * u) * 1.44269504088896341f);
-    }
+    const float t = rcp_fast(1.f + 0.35f * fabsf(z));
+    float p = -0.029108895f;
+    p = p * t + 0.14378804f; p = p * t - 0.255326897f; p = p * t + 0.158721581f; p = p * t - 0.0227904506f;
+    p = p * t + 0.105369069f; p = p * t + 0.11986912f; p = p * t + 0.139856696f; p = p * t + 0.139621705f;
+    return p * t * e;
 }
 __device__ __forceinline__ float sigmoid_fast(float z) { return rcp_fast(1.f + exp2_fast(-1.44269504088896341f * z)); }
 // z + 0.044715 z^3 scaled so that its sigmoid is (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2
@@ -65,7 +56,7 @@ template <typename T, int V, bool SLOPE> __device__ __forceinline__ void apply_a
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 float g;
-                const float q = normal_tail<T>(v[e], g), p = v[e] > 0.f ? 1.f - q : q;
+                const float q = normal_tail(v[e], g), p = v[e] > 0.f ? 1.f - q : q;
                 if (SLOPE) d[e] = p + v[e] * 0.39894228040143268f * g;
                 v[e] *= p;
             }
@@ -605,44 +596,47 @@ __global__ __launch_bounds__(256) void slope_kernel(const void* dy_, int64_t ldd
     __shared__ float sums[4][64 * V];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = (blockIdx.x * 64 + lane) * V;
-    const int64_t r0 = (int64_t)blockIdx.y * SLOPE_ROWS, r1 = r0 + SLOPE_ROWS < M ? r0 + SLOPE_ROWS : M;
     typedef Pack<T, V> P;
-    float sum[V];
+    for (int64_t chunk = blockIdx.y; chunk * SLOPE_ROWS < M; chunk += gridDim.y) {
+        const int64_t r0 = chunk * SLOPE_ROWS, r1 = r0 + SLOPE_ROWS < M ? r0 + SLOPE_ROWS : M;
+        float sum[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) sum[e] = 0.f;
-    if (n < N) {
+        for (int e = 0; e < V; ++e) sum[e] = 0.f;
+        if (n < N) {
 #pragma unroll 4
-        for (int64_t m = r0 + wave; m < r1; m += 4) {
-            const P d = *reinterpret_cast<const P*>(static_cast<const T*>(dy_) + m * ldd + n);
-            if (act != ACT_NONE) {
-                const Pack<S, V> q = *reinterpret_cast<const Pack<S, V>*>(static_cast<const S*>(slope_) + m * N + n);
-                P o;
+            for (int64_t m = r0 + wave; m < r1; m += 4) {
+                const P d = *reinterpret_cast<const P*>(static_cast<const T*>(dy_) + m * ldd + n);
+                if (act != ACT_NONE) {
+                    const Pack<S, V> q = *reinterpret_cast<const Pack<S, V>*>(static_cast<const S*>(slope_) + m * N + n);
+                    P o;
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float g = (float)d.v[e] * slope_value(q.v[e], act);
-                    sum[e] += g;
-                    o.v[e] = (T)g;
+                    for (int e = 0; e < V; ++e) {
+                        const float g = (float)d.v[e] * slope_value(q.v[e], act);
+                        sum[e] += g;
+                        o.v[e] = (T)g;
+                    }
+                    if (dz_) *reinterpret_cast<P*>(static_cast<T*>(dz_) + m * ldz + n) = o;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) sum[e] += (float)d.v[e];
+                    if (dz_) *reinterpret_cast<P*>(static_cast<T*>(dz_) + m * ldz + n) = d;        // laid out anew
                 }
-                if (dz_) *reinterpret_cast<P*>(static_cast<T*>(dz_) + m * ldz + n) = o;
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e) sum[e] += (float)d.v[e];
-                if (dz_) *reinterpret_cast<P*>(static_cast<T*>(dz_) + m * ldz + n) = d;        // laid out anew
             }
+        } else if (!VEC && dz_ && n < ldz) {                       // zeros up to whole pieces
+            for (int64_t m = r0 + wave; m < r1; m += 4) static_cast<T*>(dz_)[m * ldz + n] = (T)0.f;
         }
-    } else if (!VEC && dz_ && n < ldz) {                       // zeros up to whole pieces
-        for (int64_t m = r0 + wave; m < r1; m += 4) static_cast<T*>(dz_)[m * ldz + n] = (T)0.f;
-    }
-    if (!part) return;
+        if (!part) continue;
+        __syncthreads();                                            // the chunk before has been read
 #pragma unroll
-    for (int e = 0; e < V; ++e) sums[wave][lane * V + e] = sum[e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * V; i += 256) {
-        const int col = blockIdx.x * 64 * V + i;
-        if (col >= N) continue;
-        const float s = (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
-        if (db) static_cast<T*>(db)[col] = (T)s;                // all rows in one chunk
-        else part[(int64_t)blockIdx.y * N + col] = s;
+        for (int e = 0; e < V; ++e) sums[wave][lane * V + e] = sum[e];
+        __syncthreads();
+        for (int i = threadIdx.x; i < 64 * V; i += 256) {
+            const int col = blockIdx.x * 64 * V + i;
+            if (col >= N) continue;
+            const float s = (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
+            if (db) static_cast<T*>(db)[col] = (T)s;                // all rows in one chunk
+            else part[chunk * N + col] = s;
+        }
     }
 }
 
@@ -651,11 +645,11 @@ template <typename T>
 __global__ __launch_bounds__(256) void product_pack_kernel(const void* x, int64_t ld, int64_t rows, int cols, void* out) {
     constexpr int CE = 16 / sizeof(T);
     const int per_row = (cols + CE - 1) / CE;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows * per_row) return;
-    const int64_t r = i / per_row;
-    const int c = (int)(i - r * per_row) * CE;
-    static_cast<uint4*>(out)[i] = unaligned_chunk(static_cast<const T*>(x) + r * ld + c, cols - c);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per_row; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per_row;
+        const int c = (int)(i - r * per_row) * CE;
+        static_cast<uint4*>(out)[i] = unaligned_chunk(static_cast<const T*>(x) + r * ld + c, cols - c);
+    }
 }
 
 constexpr int JOIN_WAVES = 16;
@@ -729,8 +723,8 @@ inline bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) =
 inline int whole(int64_t n, int dt) { const int V = 16 / dtype_bytes(dt); return (int)((n + V - 1) / V * V); }      // up to whole 16-byte pieces
 
 void pack_rows(const void* x, int64_t ld, int64_t rows, int cols, int dt, void* out, hipStream_t s) {
-    const int64_t n = rows * (whole(cols, dt) / (16 / dtype_bytes(dt)));
-    with_dtype(dt, [&](auto t) { hipLaunchKernelGGL(product_pack_kernel<decltype(t)>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, x, ld, rows, cols, out); });
+    const int64_t n = rows * (whole(cols, dt) / (16 / dtype_bytes(dt))), blocks = (n + 255) / 256;
+    with_dtype(dt, [&](auto t) { hipLaunchKernelGGL(product_pack_kernel<decltype(t)>, dim3((unsigned)(blocks < (1 << 22) ? blocks : 1 << 22)), dim3(256), 0, s, x, ld, rows, cols, out); });
 }
 
 // packed: row operands have zeros behind their K values up to whole pieces
@@ -755,7 +749,7 @@ hipError_t product(ProductArgs a, int dt, bool acol, bool bcol, bool packed, voi
     if (any) p.tile = 64;
     a.splits = p.splits; a.k_split = p.k_split; a.part = static_cast<float*>(part);
     a.tiles_m = (int)((a.M + p.tile - 1) / p.tile); a.tiles_n = (a.N + p.tile - 1) / p.tile;
-    if ((int64_t)a.tiles_m * a.tiles_n > 0x3FFFFFFF) return hipErrorInvalidValue;
+    if ((int64_t)a.tiles_m * a.tiles_n > (1 << 23) - 8) return hipErrorInvalidValue;           // 2^32 threads a launch
     with_dtype(dt, [&](auto t) {
         typedef decltype(t) T;
         auto by_tile = [&](auto ac, auto bc) {
@@ -819,7 +813,8 @@ BwdWorkspace bwd_workspace(int64_t M, int N, int64_t K, int act, int dt) {
     return w;
 }
 
-bool shape_ok(int64_t M, int N, int K) { return M >= 0 && N > 0 && K > 0 && M <= (int64_t)1 << 30; }
+// widths: 16 rows of w a workgroup of 512 threads, 2^32 threads a launch
+bool shape_ok(int64_t M, int N, int K) { return M >= 0 && N > 0 && K > 0 && M <= (int64_t)1 << 30 && N <= 1 << 26 && K <= 1 << 26; }
 
 }  // namespace
 }  // namespace adx
@@ -838,7 +833,7 @@ ADX_API int adx_op_linear_residual(const void* x, int64_t ldx, const void* w, in
                                    void* stream) {
     if (!dtype_ok(dtype)) { set_error("linear_residual: unknown element type"); return ADX_EINVAL; }
     if (act < ACT_NONE || act > ACT_TANH_) { set_error("linear_residual: unknown activation"); return ADX_EINVAL; }
-    if (!shape_ok(M, N, K)) { set_error("linear_residual: needs 0 <= M <= 2^30 and positive N, K"); return ADX_EINVAL; }
+    if (!shape_ok(M, N, K)) { set_error("linear_residual: needs 0 <= M <= 2^30 and 0 < N, K <= 2^26"); return ADX_EINVAL; }
     if (M == 0) return ADX_OK;
     if (!x || !w || !y) { set_error("linear_residual: null pointer"); return ADX_EINVAL; }
     if (ldx < 0 || ldw < 0 || ldr < 0 || ldy < N) { set_error("linear_residual: negative row stride, or output rows that overlap"); return ADX_EINVAL; }
@@ -870,7 +865,7 @@ ADX_API int adx_op_linear_residual_bwd(const void* dy, int64_t ldd, const void* 
                                        void* stream) {
     if (!dtype_ok(dtype)) { set_error("linear_residual_bwd: unknown element type"); return ADX_EINVAL; }
     if (act < ACT_NONE || act > ACT_TANH_) { set_error("linear_residual_bwd: unknown activation"); return ADX_EINVAL; }
-    if (!shape_ok(M, N, K) || M == 0) { set_error("linear_residual_bwd: needs 1 <= M <= 2^30 and positive N, K"); return ADX_EINVAL; }
+    if (!shape_ok(M, N, K) || M == 0) { set_error("linear_residual_bwd: needs 1 <= M <= 2^30 and 0 < N, K <= 2^26"); return ADX_EINVAL; }
     if (!dy || (dx && !w) || (dw && !x) || (act != ACT_NONE && !slope)) { set_error("linear_residual_bwd: null pointer"); return ADX_EINVAL; }
     if (ldd < 0 || ldx < 0 || ldw < 0) { set_error("linear_residual_bwd: negative row stride"); return ADX_EINVAL; }
     const BwdWorkspace ws = bwd_workspace(M, N, K, act, dtype);
@@ -885,12 +880,11 @@ ADX_API int adx_op_linear_residual_bwd(const void* dy, int64_t ldd, const void* 
     const bool store = ws.store_dz && (dx || dw);
     const int Np = whole(N, dtype), Kp = whole(K, dtype);
     if (store || db) {
-        if (ws.chunks > 65535) { set_error("linear_residual_bwd: more than 4 million rows"); return ADX_EINVAL; }
         const bool vec = N % V == 0 && ldd % V == 0 && on16(dy) && on16(slope);
         with_dtype(dtype, [&](auto t) {
             typedef decltype(t) T;
             const int cols = vec ? 64 * V : 64, width = store ? Np : N;
-            const dim3 grid((unsigned)((width + cols - 1) / cols), (unsigned)ws.chunks);
+            const dim3 grid((unsigned)((width + cols - 1) / cols), (unsigned)(ws.chunks < 65535 ? ws.chunks : 65535));
             void* to = store ? dz : nullptr;
             float* part = db ? sums : nullptr;
             void* whole_db = ws.chunks == 1 ? db : nullptr;

@@ -13,11 +13,6 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
-template <typename T> struct Typed;
-template <> struct Typed<float> { static constexpr int V = 4; static constexpr int dt = DT_F32; };
-template <> struct Typed<__bf16> { static constexpr int V = 8; static constexpr int dt = DT_BF16; };
-template <> struct Typed<_Float16> { static constexpr int V = 8; static constexpr int dt = DT_F16; };
-
 // N elements moved as one load or store (16, 8, 4 or 2 bytes)
 template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
 

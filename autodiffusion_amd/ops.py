@@ -4,6 +4,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import operator
 from typing import Optional, Sequence
 
 import torch
@@ -298,6 +299,7 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions, inv_freq: torch.
     if rd > dh or rd == 0 or hq == 0 or (k is not None and hk == 0):
         raise ValueError(f"rope: {rd} rotated values of heads of {dh}, and at least one head")
     pos = positions if isinstance(positions, torch.Tensor) else None
+    first = operator.index(positions) if pos is None else 0
     if pos is not None and pos.dtype != torch.int64:
         raise ValueError("rope: positions are int64")
     if inplace:
@@ -306,11 +308,16 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions, inv_freq: torch.
                 raise ValueError("rope: in place needs adjacent values in a head")
             if t is not None and any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
                 raise ValueError("rope: in place needs a tensor without repeated elements")
+            if t is not None and t.requires_grad and torch.is_grad_enabled():
+                raise ValueError("rope: in place is not recorded for gradients (train.rope)")
         if k is not None and k.numel() and k.data_ptr() == q.data_ptr():
             raise ValueError("rope: q and k in place are the same memory")
     stream = stream_on(device_of("rope", q, k, pos, inv_freq))
     if inplace:
         qo, ko = q, k
+        for t in (q, k):
+            if t is not None and not t.is_inference():
+                torch.autograd.graph.increment_version(t)        # a graph that kept the old values notices
     else:
         if dh > 1 and q.stride(-1) != 1:
             q = q.contiguous()
@@ -331,7 +338,7 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions, inv_freq: torch.
     st = outer + q.stride()[:-1] + outer + qo.stride()[:-1]
     st += (0,) * 6 if k is None else outer + k.stride()[:-1] + outer + ko.stride()[:-1]
     check(_lib.load().adx_op_rope(q.data_ptr(), qo.data_ptr(), hq, None if k is None else k.data_ptr(), None if k is None else ko.data_ptr(), hk,
-                                  _Strides(*st), None if pos is None else pos.data_ptr(), pb, ps, 0 if pos is not None else int(positions),
+                                  _Strides(*st), None if pos is None else pos.data_ptr(), pb, ps, first,
                                   inv_freq.data_ptr(), amplitude, B, S, dh, rd, layout == "interleaved", inverse, dt, stream), "rope")
     return qo, ko
 

@@ -194,6 +194,9 @@ class MixtralModel(nn.Module):
         super().__init__()
         if hidden_size % num_attention_heads or num_attention_heads % num_key_value_heads or (hidden_size // num_attention_heads) % 2:
             raise ValueError("MixtralModel: hidden size divisible by the head count, head count by the key / value head count, even head width")
+        if few_token_experts and (hidden_size % 32 or intermediate_size % 32 or num_local_experts > 64 or num_experts_per_tok > 8 or
+                                  hidden_size * intermediate_size > 1 << 28):
+            raise ValueError("MixtralModel: few_token_experts needs widths that are multiples of 32, at most 64 experts and 8 of them a token")
         if hidden_size % 32 or intermediate_size % 32:
             raise ValueError("MixtralModel: hidden and expert widths must be multiples of 32")
         self.embed_tokens = nn.Module()                                  # in the checkpoint; the model is driven by embeddings

@@ -888,4 +888,6 @@ def linear_residual(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tenso
                     act: int = _lib.ACT_NONE) -> torch.Tensor:
     """``ops.linear_residual`` with gradients for x, w, bias and residual.  For the backward it keeps x, w and the
     activation's slope (in 16 bits where the tensors have 16)."""
+    if not torch.is_grad_enabled():                      # parameters want gradients, this call does not: no slope is written
+        return ops.linear_residual(x, w, bias, residual, act)
     return _LinearResidual.apply(x, w, bias, residual, act)

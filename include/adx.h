@@ -305,8 +305,8 @@ int adx_op_moe_block(const float* x, const float* res, const float* router_w, co
 int adx_op_rope(const void* q, void* q_out, int heads_q, const void* k, void* k_out, int heads_k, const int64_t* strides_host,
                 const int64_t* positions, int64_t pos_stride_b, int64_t pos_stride_s, int64_t pos0, const double* inv_freq, float amplitude,
                 int B, int S, int dh, int rotary_dim, int interleaved, int inverse, int dtype, void* stream);
-/* y[M][N] = act(x[M][K] w[N][K]^T + bias[N]) + res[M][N]; bias, res nullable; all tensors of one element type; row strides (elements)
- * ldx, ldw, ldr, ldy >= N, adjacent values in a row (ldr = 0: one row for all).  act: ADX_ACT_NONE .. ADX_ACT_TANH.  slope (nullable,
+/* y[M][N] = act(x[M][K] w[N][K]^T + bias[N]) + res[M][N], M <= 2^30, N and K <= 2^26; bias, res nullable; all tensors of one element
+ * type, adjacent values in a row; row strides (elements) ldy >= N and ldx, ldw, ldr >= 0 (0: one row for all).  act: ADX_ACT_NONE .. ADX_ACT_TANH.  slope (nullable,
  * [M][N] contiguous) receives what the gradient needs for act != ADX_ACT_NONE, act' of the sum: fp32 values for fp32 tensors; for 16-bit
  * tensors uint16 codes q of (q - 8192) / 32768 (0: NaN; LeakyReLU's 8520 stands for 0.01 itself).
  * y and slope overlap no input, except that y may be res itself (same pointer and stride).  M = 0 does nothing.
@@ -321,7 +321,7 @@ size_t adx_linear_residual_bwd_ws_bytes(int64_t M, int N, int K, int act, int dt
 int adx_op_linear_residual_bwd(const void* dy, int64_t ldd, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* slope, void* dx,
                                void* dw, void* db, int64_t M, int N, int K, int act, int dtype, void* workspace, size_t workspace_bytes,
                                void* stream);
-/* adx_op_moe_block for a few tokens (1 <= T <= 64; d, inter multiples of 32): the same expert layer in two kernels (three where the
+/* adx_op_moe_block for a few tokens (1 <= T <= 64; d, inter multiples of 32, d * inter <= 2^28; E <= 64, top_k <= 8): the same expert layer in two kernels (three where the
  * routing is large) that read the chosen experts' weights once.  x, res (nullable), y: [T][d] of act_type; router_w [E][d] fp32; w13, w2 as
  * for adx_op_moe_block under `precision`: fp32 tokens with ADX_PREC_F32, BF16, BF16X3 or F16 (fp16 bits) weights, bf16 tokens with
  * ADX_PREC_BF16, fp16 tokens with ADX_PREC_F16.  Tokens and hidden values are not rounded below their fp32 accuracy (16-bit act_type:

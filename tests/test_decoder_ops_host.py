@@ -30,6 +30,7 @@ def test_rope_abi_refusals():
         refused(call(**bad), b"even rotary width")
     refused(call(dh=8192, rd=8192), b"4096")
     refused(call(qo=FAKE, st=(C.c_int64 * 12)(64, 64, 64, 128, 128, 128, 0, 0, 0, 0, 0, 0)), b"in place")
+    refused(call(B=1 << 20, S=1 << 20, hq=4096), b"too many tokens")
     assert call(B=0) == 0 and call(S=0) == 0                        # no tokens: nothing to do
 
 
@@ -44,7 +45,7 @@ def test_linear_residual_abi_refusals():
     refused(call(dt=3), b"element type")
     refused(call(act=7), b"activation")
     refused(call(act=-1), b"activation")
-    for bad in (dict(M=-1), dict(N=0), dict(K=0), dict(M=(1 << 30) + 1)):
+    for bad in (dict(M=-1), dict(N=0), dict(K=0), dict(M=(1 << 30) + 1), dict(N=(1 << 26) + 1, ldy=1 << 27), dict(K=(1 << 26) + 1)):
         refused(call(**bad), b"needs 0 <= M")
     refused(call(ldy=63), b"overlap")
     refused(call(ldx=-1), b"negative")
@@ -67,7 +68,8 @@ def test_linear_residual_bwd_abi_refusals():
         refused(call(**bad), b"null pointer")
     refused(call(dt=-1), b"element type")
     refused(call(act=9), b"activation")
-    refused(call(M=0), b"needs 1 <= M")
+    for bad in (dict(M=0), dict(N=(1 << 26) + 1), dict(K=(1 << 26) + 1)):
+        refused(call(**bad), b"needs 1 <= M")
     need = lib.adx_linear_residual_bwd_ws_bytes(100, 64, 64, 2, BF16)
     assert need >= 100 * 64 * 2
     refused(call(n=need - 1), b"workspace")
@@ -82,7 +84,8 @@ def test_moe_few_abi_refusals():
 
     for bad in (dict(x=None), dict(router=None), dict(w13=None), dict(w2=None), dict(ws=None), dict(y=None)):
         refused(call(**bad), b"null pointer")
-    for bad in (dict(T=0), dict(T=65), dict(d=48), dict(inter=40), dict(E=65), dict(E=0), dict(k=9, E=16), dict(k=0), dict(E=2, k=3), dict(d=0)):
+    for bad in (dict(T=0), dict(T=65), dict(d=48), dict(inter=40), dict(E=65), dict(E=0), dict(k=9, E=16), dict(k=0), dict(E=2, k=3), dict(d=0),
+                dict(d=1 << 15, inter=(1 << 13) + 32)):
         refused(call(**bad), b"1 <= T <= 64")
     for at, prec in ((BF16, 0), (BF16, 4), (F16, 1), (F16, 0), (F32, 3), (3, 0), (BF16, 2)):
         refused(call(at=at, prec=prec), b"tokens with")
@@ -100,6 +103,10 @@ def test_python_refusals():
         args = dict(q=q, k=None, positions=0, inv_freq=w, layout="half", inplace=False) | bad
         with pytest.raises(ValueError):
             ops.rope(args["q"], args["k"], args["positions"], args["inv_freq"], layout=args["layout"], inplace=args["inplace"])
+    with pytest.raises(TypeError):
+        ops.rope(q, None, 1.5, w)
+    with pytest.raises(ValueError, match="gradients"):
+        ops.rope(q.clone().requires_grad_(), None, 0, w, inplace=True)
     with pytest.raises(_lib.AdxError, match="device memory"):
         ops.rope(q, None, 0, w)
     for bad in (dict(rotary_dim=7), dict(theta=0.0), dict(factor=0.0), dict(scaling="other"), dict(scaling="base", rotary_dim=2),
@@ -129,3 +136,8 @@ def test_python_refusals():
             str_backbone.moe_few(**(ok | bad))
     with pytest.raises(_lib.AdxError, match="device memory"):
         str_backbone.moe_few(**ok)
+    for bad in (dict(hidden_size=48, num_attention_heads=3, num_key_value_heads=3), dict(intermediate_size=80), dict(num_local_experts=65),
+                dict(num_local_experts=16, num_experts_per_tok=9)):
+        with pytest.raises(ValueError, match="few_token_experts"):
+            str_backbone.MixtralModel(**(dict(hidden_size=64, intermediate_size=96, num_hidden_layers=1, num_attention_heads=4, num_key_value_heads=4,
+                                              vocab_size=8, few_token_experts=True) | bad))

@@ -61,6 +61,8 @@ def rope_exact(x, pos, w, amp, layout, inverse=False):
     (3, 5, 3, 3, 7, 6, 40),                # odd head width
     (1, 2, 2, 1, 520, 514, 2 ** 31 - 2),   # wide heads, the farthest positions
     (2, 1030, 4, 1, 128, 128, 0),
+    (1, 1, 70, 5, 256, 256, 12),           # one token of many heads: several workgroups a token
+    (3, 2, 2, 1, 1100, 1030, 9),           # more pieces a head than threads, with a tail
 ])
 def test_rope(dev, kind, layout, B, S, Hq, Hk, dh, rd, first):
     from autodiffusion_amd import ops
@@ -290,6 +292,42 @@ def test_linear_residual_bwd_large(dev):
         within(dx, d @ w.double(), (N + 2) * U24 * d.abs() @ aw, kind, "dx")
         within(dw, d.t() @ x.double(), (M + 2) * U24 * d.abs().t() @ ax, kind, "dw")
         within(db, d.sum(0), (M + 2) * U24 * d.abs().sum(0), kind, "db")
+
+
+def test_linear_residual_bwd_of_many_rows(dev):
+    """More 64-row chunks than a launch has groups (65535): db and dw of 4.2 million rows."""
+    from autodiffusion_amd import ops
+    M, N, K = 65535 * 64 + 77, 9, 8
+    g = torch.Generator(device="cuda").manual_seed(21)
+    x, w, dy = (torch.randn(*s, generator=g, device=dev).bfloat16() for s in ((M, K), (N, K), (M, N)))
+    y, slope = ops.linear_residual(x, w, act=1, keep_slope=True)
+    dx, dw, db = ops.linear_residual_bwd(dy, x, w, slope, act=1)
+    dz = dy.double() * slope_values(slope, "relu", "bf16")
+    assert torch.equal(slope_values(slope, "relu", "bf16")[-100:], (y[-100:] > 0).double())
+    # sums of at most 8200 partial sums of at most 4100 terms each way; relu's slope is 0 or 1: dz is exact
+    e = 12300 * U24
+    within(dw, dz.t() @ x.double(), e * dz.abs().t() @ x.double().abs(), "bf16", "dw")
+    within(db, dz.sum(0), e * dz.abs().sum(0), "bf16", "db")
+    within(dx[-200:], dz[-200:] @ w.double(), (N + 2) * U24 * dz[-200:].abs() @ w.double().abs(), "bf16", "dx")
+
+
+def test_no_gradient_mode(dev):
+    """Without gradients the training forms give the same values and record nothing; a rotation in place is seen by a graph that kept the tensor."""
+    from autodiffusion_amd import ops, train
+    g = torch.Generator().manual_seed(22)
+    x, w = rand(g, 70, 64), rand(g, 64, 64).requires_grad_()
+    with torch.no_grad():
+        y = train.linear_residual(x, w, act=2)
+    assert not y.requires_grad and torch.equal(y, train.linear_residual(x, w, act=2).detach())
+    freq, _ = ops.rope_frequencies(16)
+    kept = rand(g, 1, 5, 4, 16)
+    loss = (rand(g, 1, 5, 4, 16).requires_grad_() * kept).sum()
+    ops.rope(kept, None, 0, freq, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        t = kept.clone()
+        assert torch.equal(ops.rope(t, None, 3, freq, inplace=True)[0], ops.rope(kept, None, 3, freq)[0])
 
 
 def directional(f, leaves, grads, gen):
