@@ -311,6 +311,34 @@ def test_linear_residual_bwd_of_many_rows(dev):
     within(dx[-200:], dz[-200:] @ w.double(), (N + 2) * U24 * dz[-200:].abs() @ w.double().abs(), "bf16", "dx")
 
 
+def test_offsets_beyond_32_bits(dev):
+    """Tensors of more than 2^31 values: the last rows of the product, of its gradients and of a rotation."""
+    from autodiffusion_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(23)
+    M, N, K = 1_050_001, 2056, 16
+    x, w = (torch.randn(*s, generator=g, device=dev).bfloat16() for s in ((M, K), (N, K)))
+    y, slope = ops.linear_residual(x, w, act=1, keep_slope=True)
+    want, e, _, _ = linear_exact(x[-70:], w, None, None, "relu")
+    within(y[-70:], want, e, "bf16", "y")
+    assert torch.equal(slope_values(slope[-70:], "relu", "bf16"), (y[-70:] > 0).double())
+    dy = y.zero_()
+    dy[-70:] = torch.randn(70, N, generator=g, device=dev).bfloat16()
+    dx, dw, db = ops.linear_residual_bwd(dy, x, w, slope, act=1)
+    dz, xe = dy[-70:].double() * slope_values(slope[-70:], "relu", "bf16"), x[-70:].double()
+    within(dx[-70:], dz @ w.double(), (N + 2) * U24 * dz.abs() @ w.double().abs(), "bf16", "dx")
+    assert not dx[:-70].any()
+    within(dw, dz.t() @ xe, 72 * U24 * dz.abs().t() @ xe.abs(), "bf16", "dw")
+    within(db, dz.sum(0), 72 * U24 * dz.abs().sum(0), "bf16", "db")
+    del y, slope, dy, dx, x
+    tokens, heads, dh = 270_001, 64, 128
+    q = torch.empty(tokens, heads, dh, dtype=torch.bfloat16, device=dev)
+    q[-9:] = torch.randn(9, heads, dh, generator=g, device=dev).bfloat16()
+    freq, amp = ops.rope_frequencies(dh)
+    tail = q[-9:].clone()
+    ops.rope(q, None, 3, freq, amp, inplace=True)
+    assert torch.equal(q[-9:], ops.rope(tail, None, 3 + tokens - 9, freq, amp)[0])
+
+
 def test_no_gradient_mode(dev):
     """Without gradients the training forms give the same values and record nothing; a rotation in place is seen by a graph that kept the tensor."""
     from autodiffusion_amd import ops, train
