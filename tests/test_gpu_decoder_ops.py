@@ -222,6 +222,21 @@ def test_linear_residual_strides(dev):
     assert ops.linear_residual(rand(g, 0, 16), rand(g, 8, 16)).shape == (0, 8)
 
 
+@pytest.mark.parametrize("kind,M,N,K", [("bf16", 3000, 5000, 64), ("fp16", 2000, 2056, 200), ("fp32", 700, 516, 64), ("bf16", 129, 127, 2050), ("bf16", 100, 64, 8192), ("fp16", 17, 100, 36)])
+def test_linear_residual_onto_the_residual(dev, kind, M, N, K):
+    """The raw entry with y in place of the residual (every tile size, a split sum, rows that fill no piece): the bits of the call beside it."""
+    from autodiffusion_amd import _lib, ops
+    g = torch.Generator().manual_seed(M + K)
+    x, w, b, res = rand(g, M, K, kind=kind), rand(g, N, K, kind=kind, scale=K ** -0.5), rand(g, N, kind=kind), rand(g, M, N, kind=kind)
+    want = ops.linear_residual(x, w, b, res, act=5)
+    lib, dt = _lib.load(), _lib.DTYPES[TYPES[kind]]
+    need = lib.adx_linear_residual_ws_bytes(M, N, K, dt)
+    ws = torch.empty(need + 16, dtype=torch.uint8, device=dev)
+    _lib.check(lib.adx_op_linear_residual(x.data_ptr(), K, w.data_ptr(), K, b.data_ptr(), res.data_ptr(), N, None, res.data_ptr(), N, M, N, K, 5, dt, ws.data_ptr(),
+                                          need, torch.cuda.current_stream().cuda_stream), "linear_residual")
+    assert torch.equal(res, want)
+
+
 def test_linear_residual_not_finite(dev):
     """An infinity or NaN reaches its own row alone, also through activations and behind ragged ends."""
     from autodiffusion_amd import ops
