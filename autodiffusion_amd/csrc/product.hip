@@ -115,11 +115,13 @@ __device__ __forceinline__ Pack<T, V> residual_at(const ProductArgs& a, int64_t 
     return *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.res) + m * a.ldr + n);
 }
 template <typename T, int V>
-__device__ __forceinline__ void activate(const ProductArgs& a, int64_t m, int n, float (&v)[V]) {
+__device__ __forceinline__ Pack<T, V> bias_at(const ProductArgs& a, int n) {
+    return *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.bias) + n);
+}
+template <typename T, int V>
+__device__ __forceinline__ void activate(const ProductArgs& a, int64_t m, int n, float (&v)[V], const Pack<T, V>& b) {
     typedef typename Slope<T>::type S;
-    typedef Pack<T, V> P;
     if (a.bias) {
-        const P b = *reinterpret_cast<const P*>(static_cast<const T*>(a.bias) + n);
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] += (float)b.v[e];
     }
@@ -142,7 +144,9 @@ __device__ __forceinline__ void put(const ProductArgs& a, int64_t m, int n, cons
 }
 template <typename T, int V>
 __device__ __forceinline__ void finish(const ProductArgs& a, int64_t m, int n, float (&v)[V]) {
-    activate<T, V>(a, m, n, v);
+    Pack<T, V> b{};
+    if (a.bias) b = bias_at<T, V>(a, n);
+    activate<T, V>(a, m, n, v, b);
     if (a.res) {
         const Pack<T, V> r = residual_at<T, V>(a, m, n);
 #pragma unroll
@@ -245,8 +249,9 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, f32x16_t (&acc)
     constexpr int NW = FJ * 32, EP_LD = NW + 4, V = 16 / sizeof(T), LPR = NW / V, RPI = 64 / LPR;   // lanes of a row, rows of one pass
     float* patch = reinterpret_cast<float*>(smem) + wave * 32 * EP_LD;
     const int n = n_wave + (lane % LPR) * V;
-    // The residual of the first 64 rows is in registers (the fragments' are free) before the first store, later rows follow 64 behind: a load
-    // is waited for with every store issued before it.  Read one pass of 8 rows ahead, 6984 x 4096 x 1024 bf16 took 97 us instead of 84.
+    // Loads are waited for with every store issued before them, so none stands between stores: the bias of the lane's columns and the residual of the
+    // first 64 rows are in registers (the fragments' are free) before the first store, later rows follow 64 behind.  With both read where they are
+    // used (the residual a pass of 8 rows ahead) 6984 x 4096 x 1024 bf16 takes 97 us instead of 80.
     // Activated sums go back to LDS, so that only the addition of the residual is unrolled, not the activations.
     constexpr int PASSES = 32 / RPI, HELD = FI <= 2 ? FI : 2;
     const bool with_res = a.res && a.vec && a.splits <= 1;
@@ -267,6 +272,8 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, f32x16_t (&acc)
             v[e] = f.x; v[e + 1] = f.y; v[e + 2] = f.z; v[e + 3] = f.w;
         }
     };
+    Pack<T, V> bias{};
+    if (a.bias && a.vec) bias = bias_at<T, V>(a, n < a.N ? n : 0);
     if (with_res)
 #pragma unroll
         for (int i = 0; i < HELD; ++i) hold(i);
@@ -311,7 +318,7 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, f32x16_t (&acc)
 #pragma unroll
                         for (int e = 0; e < V; e += 4) *reinterpret_cast<float4*>(o + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                     } else {
-                        activate<T, V>(a, m, n, v);
+                        activate<T, V>(a, m, n, v, bias);
                         put<T, V>(a, m, n, v);
                     }
                 }
@@ -323,7 +330,7 @@ __device__ __forceinline__ void store_tile(const ProductArgs& a, f32x16_t (&acc)
                 const int64_t m = m_wave + i * 32 + r;
                 float v[V];
                 get(r, v);
-                if (m < a.M && n < a.N) activate<T, V>(a, m, n, v);
+                if (m < a.M && n < a.N) activate<T, V>(a, m, n, v, bias);
 #pragma unroll
                 for (int e = 0; e < V; e += 4) *reinterpret_cast<float4*>(sums(r) + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
             }
