@@ -860,9 +860,9 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions, inv_freq: torch.
 
 class _LinearResidual(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, bias, residual, act_code):
-        need = ctx.needs_input_grad
-        grad = need[0] or need[1] or need[2]
+    def forward(ctx, x, w, bias, residual, act_code, recorded):
+        need = ctx.needs_input_grad                      # what the inputs want, also where no graph is recorded
+        grad = recorded and (need[0] or need[1] or need[2])
         slope = None
         if grad and act_code != _lib.ACT_NONE:
             y, slope = ops.linear_residual(x, w, bias, residual, act_code, True)
@@ -881,13 +881,12 @@ class _LinearResidual(torch.autograd.Function):
         if need[0] or need[1] or need[2]:
             x, w, slope = ctx.saved_tensors
             dx, dw, db = ops.linear_residual_bwd(dy, x, w, slope, ctx.act_code, need[0], need[1], need[2])
-        return dx, dw, db, dy if need[3] else None, None
+        return dx, dw, db, dy if need[3] else None, None, None
 
 
 def linear_residual(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
                     act: int = _lib.ACT_NONE) -> torch.Tensor:
     """``ops.linear_residual`` with gradients for x, w, bias and residual.  For the backward it keeps x, w and the
-    activation's slope (in 16 bits where the tensors have 16)."""
-    if not torch.is_grad_enabled():                      # parameters want gradients, this call does not: no slope is written
-        return ops.linear_residual(x, w, bias, residual, act)
-    return _LinearResidual.apply(x, w, bias, residual, act)
+    activation's slope (in 16 bits where the tensors have 16); without gradients nothing.  Forward-mode derivatives are refused, with gradients
+    enabled or not."""
+    return _LinearResidual.apply(x, w, bias, residual, act, torch.is_grad_enabled())
