@@ -852,7 +852,12 @@ class _Rope(torch.autograd.Function):
 
 
 def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions, inv_freq: torch.Tensor, amplitude: float = 1.0, layout: str = "half"):
-    """``ops.rope`` with gradients: (q', k') -- (q', None) without k.  The gradient is the transposed rotation of the outputs' gradients."""
+    """``ops.rope`` with gradients for q and k: (q', k') -- (q', None) without k.  The gradient is the transposed rotation of the outputs'
+    gradients.  Frequencies and amplitude have none: ones that require grad are refused while a graph is recorded."""
+    if torch.is_grad_enabled():
+        for what, t in (("inv_freq", inv_freq), ("amplitude", amplitude)):
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                raise NotImplementedError(f"rope: the training path computes no gradient for `{what}` (it requires grad): detach it")
     if k is None:
         return _Rope.apply(q, None, positions, inv_freq, amplitude, layout), None
     return _Rope.apply(q, k, positions, inv_freq, amplitude, layout)
