@@ -20,6 +20,7 @@ PREC_F32, PREC_BF16, PREC_BF16X3, PREC_F16X2, PREC_F16 = 0, 1, 2, 3, 4
 PRECISIONS = {"fp32": PREC_F32, "bf16": PREC_BF16, "bf16x3": PREC_BF16X3, "f16x2": PREC_F16X2, "f16": PREC_F16}
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # ADX_DT_*: element types of the operators that take more than fp32
 VARIANT_A, VARIANT_DIT, VARIANT_MMDIT = 0, 1, 2
+INT_MAX = 2 ** 31 - 1                   # ctypes passes a C int's low 32 bits without a word: sizes are compared before the call
 FLAG_NORMALIZE, FLAG_RESIDUAL, FLAG_INIT_ZERO, FLAG_NO_GRAPH, FLAG_KEEP_MAPS = 1, 2, 4, 8, 16
 
 EXPORTS = [

@@ -10,7 +10,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import DTYPES, StepCoef, check, current_stream, device_of, f32c, on_data_device, ptr, stream_on
+from ._lib import DTYPES, INT_MAX, StepCoef, check, current_stream, device_of, f32c, on_data_device, ptr, stream_on
 
 
 def timestep_embedding(t: torch.Tensor, dim: int) -> torch.Tensor:
@@ -282,7 +282,7 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions, inv_freq: torch.
     ``positions``: an int (token s of every item at positions + s) or an int64 tensor that broadcasts to the token axes; ``inv_freq`` (rd / 2,)
     fp64 and ``amplitude`` as ``rope_frequencies`` gives them: the first rd <= dh values of a head are rotated, the others copied.  ``layout``:
     "half" pairs (j, j + rd / 2), "interleaved" (2 j, 2 j + 1).  fp32, bf16 or fp16; any strides with adjacent values in a head (a slice of
-    a fused q / k / v product, heads before tokens as a transposed view).  ``inverse`` applies the transpose -- the gradient.
+    a fused q / k / v product, heads before tokens as a transposed view); every axis below 2^31.  ``inverse`` applies the transpose -- the gradient.
     ``inplace`` writes into q and k, which must not overlap each other."""
     if layout != "half" and layout != "interleaved":
         raise ValueError(f"rope: unknown layout {layout!r}")
@@ -298,8 +298,12 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions, inv_freq: torch.
     hk = 0 if k is None else k.shape[-2]
     if rd > dh or rd == 0 or hq == 0 or (k is not None and hk == 0):
         raise ValueError(f"rope: {rd} rotated values of heads of {dh}, and at least one head")
+    if shape[0] > INT_MAX or shape[-3] > INT_MAX or hq > INT_MAX or hk > INT_MAX or dh > INT_MAX:
+        raise ValueError("rope: items, tokens, heads and head width are below 2^31 each")
     pos = positions if isinstance(positions, torch.Tensor) else None
     first = operator.index(positions) if pos is None else 0
+    if not -(1 << 62) <= first <= 1 << 62:
+        raise ValueError("rope: positions are int64")
     if pos is not None and pos.dtype != torch.int64:
         raise ValueError("rope: positions are int64")
     if inplace:
@@ -364,6 +368,13 @@ def _on_pieces(t: torch.Tensor, ld: int):
     return t, ld
 
 
+def _linear_sizes(what: str, N: int, K: int, act: int) -> None:
+    if N > 1 << 26 or K > 1 << 26:
+        raise ValueError(f"{what}: widths of at most 2^26")
+    if not _lib.ACT_NONE <= act <= _lib.ACT_TANH:
+        raise ValueError(f"{what}: unknown activation {act}")
+
+
 @functools.lru_cache(maxsize=4096)
 def _linear_residual_bytes(M: int, N: int, K: int, dt: int, act: int = -1) -> int:
     lib = _lib.load()
@@ -385,6 +396,7 @@ def linear_residual(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tenso
     N, K = w.shape
     if x.shape[-1] != K or N == 0 or K == 0:
         raise ValueError("linear_residual: x (..., K) and w (N, K)")
+    _linear_sizes("linear_residual", N, K, act)
     out_shape = (*x.shape[:-1], N)
     if (bias is not None and bias.shape != (N,)) or (residual is not None and residual.shape != out_shape):
         raise ValueError("linear_residual: bias (N,) and residual of the output's shape")
@@ -423,6 +435,7 @@ def linear_residual_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, slop
     N, K = w.shape
     if x.shape[-1] != K or dy.shape != (*x.shape[:-1], N) or (slope is not None and slope.shape != dy.shape):
         raise ValueError("linear_residual_bwd: x (..., K), w (N, K), dy and slope (..., N)")
+    _linear_sizes("linear_residual_bwd", N, K, act)
     if act != _lib.ACT_NONE and slope is None:
         raise ValueError("linear_residual_bwd: the activation's gradient needs slope (linear_residual with keep_slope)")
     stream = stream_on(device_of("linear_residual_bwd", dy, x, w, slope))

@@ -32,7 +32,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib, ops
-from ._lib import DTYPES, check, current_stream, device_of, f32c, on_data_device, ptr, stream_on
+from ._lib import DTYPES, INT_MAX, check, current_stream, device_of, f32c, on_data_device, ptr, stream_on
 from .raster_encoder import NuplanRasterizeEncoder, _add, _tanh
 from .refiner import _Lin
 from .trajectory_decoder import TrajectoryDecoder
@@ -110,6 +110,8 @@ def moe_few(x: torch.Tensor, res: Optional[torch.Tensor], router_w: torch.Tensor
     if kinds is None:
         raise ValueError(f"moe_few: no form of the weights under precision {precision!r}")
     T, d = x.shape
+    if T > INT_MAX or d > INT_MAX or not 1 <= top_k <= n_experts <= INT_MAX or inter > INT_MAX:
+        raise ValueError("moe_few: 1 <= top_k <= n_experts, and sizes below 2^31")
     if router_w.dtype != torch.float32 or router_w.shape != (n_experts, d):
         raise ValueError("moe_few: router_w (E, d) fp32")
     n = n_experts * inter * d * (2 if precision == "bf16x3" else 1)

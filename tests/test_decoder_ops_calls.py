@@ -4,7 +4,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fw
 
-from autodiffusion_amd import ops, train
+from autodiffusion_amd import ops, str_backbone, train
 
 
 @pytest.fixture
@@ -53,3 +53,38 @@ def test_rope_refuses_gradients_of_its_frequencies(monkeypatch):
     for enabled in (True, False):
         with torch.set_grad_enabled(enabled), fw.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
             train.rope(q.detach(), None, 0, fw.make_dual(w, torch.ones_like(w)))
+
+
+WRAP = 2 ** 32                                                       # what a C int drops
+
+
+def huge(*shape, dtype=torch.bfloat16):
+    """A tensor of any shape in one value's memory."""
+    return torch.zeros(1, dtype=dtype).expand(shape)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """Not passed on as their low 32 bits: tokens that nobody would have turned, columns that nobody would have computed."""
+    w = torch.ones(1, dtype=torch.float64)
+    for q, k in ((huge(WRAP, 1, 2), None), (huge(1, WRAP + 1, 1, 2), None), (huge(WRAP + 1, 1, 1, 2), None), (huge(4, WRAP + 1, 2), None),
+                 (huge(4, 1, WRAP + 2), None), (huge(4, 1, 2), huge(4, WRAP + 1, 2)), (huge(2 ** 31, 1, 2), None)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            ops.rope(q, k, 0, w)
+    for first in (2 ** 64 + 5, -2 ** 64):
+        with pytest.raises(ValueError, match="int64"):
+            ops.rope(huge(4, 1, 2), None, first, w)
+    x, wt = huge(5, 16), huge(8, 16)
+    for a, b in ((x, huge(WRAP + 128, 16)), (huge(5, WRAP + 16), huge(8, WRAP + 16)), (x, huge((1 << 26) + 1, 16))):
+        with pytest.raises(ValueError, match="2\\^26"):
+            ops.linear_residual(a, b)
+        with pytest.raises(ValueError, match="2\\^26"):
+            ops.linear_residual_bwd(huge(5, b.shape[0]), a, b)
+    for act in (WRAP, WRAP + 5, 7, -1):
+        with pytest.raises(ValueError, match="activation"):
+            ops.linear_residual(x, wt, act=act)
+        with pytest.raises(ValueError, match="activation"):
+            ops.linear_residual_bwd(huge(5, 8), x, wt, huge(5, 8, dtype=torch.int16), act=act)
+    ok = dict(x=torch.zeros(4, 32), res=None, router_w=torch.zeros(8, 32), w13=torch.zeros(8, 128, 32), w2=torch.zeros(8, 32, 64), inter=64, n_experts=8, top_k=2)
+    for bad in (dict(top_k=WRAP + 2), dict(top_k=2 - WRAP), dict(top_k=0), dict(top_k=9), dict(x=huge(WRAP + 4, 32, dtype=torch.float32))):
+        with pytest.raises(ValueError, match="top_k"):
+            str_backbone.moe_few(**(ok | bad))
