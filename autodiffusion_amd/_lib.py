@@ -18,6 +18,7 @@ LIB_PATH = os.environ.get("ADX_LIB_PATH") or os.path.join(_HERE, "libadx.so")   
 ACT_NONE, ACT_RELU, ACT_GELU_ERF, ACT_GELU_TANH, ACT_LEAKY, ACT_SILU, ACT_TANH = range(7)     # ACT_TANH: adx_op_act only
 PREC_F32, PREC_BF16, PREC_BF16X3, PREC_F16X2, PREC_F16 = 0, 1, 2, 3, 4
 PRECISIONS = {"fp32": PREC_F32, "bf16": PREC_BF16, "bf16x3": PREC_BF16X3, "f16x2": PREC_F16X2, "f16": PREC_F16}
+SLOPE_F32 = 0x100                       # or-ed to the activation of linear_residual and its backward: fp32 slopes for every type
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # ADX_DT_*: element types of the operators that take more than fp32
 VARIANT_A, VARIANT_DIT, VARIANT_MMDIT = 0, 1, 2
 INT_MAX = 2 ** 31 - 1                   # ctypes passes a C int's low 32 bits without a word: sizes are compared before the call

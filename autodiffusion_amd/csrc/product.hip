@@ -50,7 +50,13 @@ template <typename T, int V, bool SLOPE> __device__ __forceinline__ void apply_a
             break;
         case ACT_TANH_:
 #pragma unroll
-            for (int e = 0; e < V; ++e) { v[e] = tanhf(v[e]); if (SLOPE) d[e] = 1.f - v[e] * v[e]; }
+            for (int e = 0; e < V; ++e) {
+                if (SLOPE) {                                       // 1 - tanh^2 as 4 q / (1 + q)^2, q = exp(-2 |z|): the difference has no digits left beyond |z| = 9
+                    const float q = exp2_fast(-2.88539008177792682f * fabsf(v[e])), r = rcp_fast(1.f + q);
+                    d[e] = 4.f * q * r * r;
+                }
+                v[e] = tanhf(v[e]);
+            }
             break;
         case ACT_GELU_ERF:
 #pragma unroll
@@ -79,12 +85,12 @@ template <typename T, int V, bool SLOPE> __device__ __forceinline__ void apply_a
     }
 }
 
-// What the forward keeps for the gradient is the activation's slope, not its argument: the backward needs no exponentials, and in 16
-// bits a slope (-0.13 .. 1.13) fits to 2^-16 as a fixed-point number, where an argument rounded to bf16 moves the gradient as much
-// as the rounding of dz does.  fp32 tensors keep it as it is.  Codes: q stands for (q - 8192) / 32768, 0 for NaN (what the conversion of
-// one gives), and LeakyReLU's two for 1 and 0.01 themselves.
-template <typename T> struct Slope { typedef unsigned short type; };
-template <> struct Slope<float> { typedef float type; };
+// What the forward keeps for the gradient is the activation's slope, not its argument: the backward needs no exponentials.  In fp32
+// a slope has its relative accuracy down to the smallest ones: a unit in saturation (GELU at -5: -7e-6) learns from those alone.  16-bit tensors
+// may keep codes of half the size instead: q stands for (q - 8192) / 32768, 0 for NaN (what the conversion of one gives), and LeakyReLU's
+// two for 1 and 0.01 themselves -- exact for ReLU and LeakyReLU; of the smooth activations slopes below 2^-16 vanish.
+template <typename T> struct Code { typedef unsigned short type; };
+template <> struct Code<float> { typedef float type; };
 __device__ __forceinline__ void set_code(float d, float& q) { q = d; }
 __device__ __forceinline__ void set_code(float d, unsigned short& q) { q = (unsigned short)(unsigned)(d * 32768.f + 8192.5f); }
 __device__ __forceinline__ float slope_value(float q, int act) { return q; }
@@ -100,7 +106,7 @@ struct ProductArgs {
     int64_t M; int N; int64_t K;             // C is M x N, K is summed
     int64_t own_a; int own_b;                // column operands: values of their own index that may be read (M, N, or padded to whole pieces)
     const void* bias; const void* res; int64_t ldr;
-    void* slope;                             // [M][N]: the activation's slope (for the gradient), Slope<T>
+    void* slope; bool slope_f32;             // [M][N]: the activation's slope (for the gradient), fp32 or Code<T>
     void* y; int64_t ldy;
     int act;
     int splits; int64_t k_split;             // K range of one split (a multiple of the K step)
@@ -118,9 +124,15 @@ template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> bias_at(const ProductArgs& a, int n) {
     return *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.bias) + n);
 }
+template <typename S, int V>
+__device__ __forceinline__ void put_slopes(const ProductArgs& a, int64_t m, int n, const float (&d)[V]) {
+    Pack<S, V> q;
+#pragma unroll
+    for (int e = 0; e < V; ++e) set_code(d[e], q.v[e]);
+    *reinterpret_cast<Pack<S, V>*>(static_cast<S*>(a.slope) + m * a.N + n) = q;
+}
 template <typename T, int V>
 __device__ __forceinline__ void activate(const ProductArgs& a, int64_t m, int n, float (&v)[V], const Pack<T, V>& b) {
-    typedef typename Slope<T>::type S;
     if (a.bias) {
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] += (float)b.v[e];
@@ -128,10 +140,8 @@ __device__ __forceinline__ void activate(const ProductArgs& a, int64_t m, int n,
     float d[V];
     if (a.slope) {
         apply_act<T, V, true>(v, d, a.act);
-        Pack<S, V> q;
-#pragma unroll
-        for (int e = 0; e < V; ++e) set_code(d[e], q.v[e]);
-        *reinterpret_cast<Pack<S, V>*>(static_cast<S*>(a.slope) + m * a.N + n) = q;
+        if (a.slope_f32) put_slopes<float, V>(a, m, n, d);
+        else put_slopes<typename Code<T>::type, V>(a, m, n, d);
     } else apply_act<T, V, false>(v, d, a.act);
 }
 template <typename T, int V>
@@ -637,10 +647,9 @@ __global__ __launch_bounds__(64 * NWAVES) void product_few_kernel(const ProductA
 // unrounded dz (joined in chunk order: no atomics).
 constexpr int SLOPE_ROWS = 64;
 
-template <typename T, bool VEC>
+template <typename T, typename S, bool VEC>
 __global__ __launch_bounds__(256) void slope_kernel(const void* dy_, int64_t ldd, const void* slope_, void* dz_, int ldz, float* part, void* db, int64_t M, int N, int act) {
     constexpr int V = VEC ? 16 / sizeof(T) : 1, ROWS = V == 8 ? 2 : 4;
-    typedef typename Slope<T>::type S;
     __shared__ float sums[4][64 * V];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = (blockIdx.x * 64 + lane) * V;
@@ -769,7 +778,9 @@ void launch_few(const ProductArgs& a, bool aligned, hipStream_t s) {
     else hipLaunchKernelGGL((product_few_kernel<T, MT, NT, NWAVES, false>), grid, dim3(64 * NWAVES), 0, s, a);
 }
 
-inline bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool on(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
+inline bool on16(const void* p) { return on(p, 16); }
+constexpr int SLOPE_F32 = 0x100;             // ADX_SLOPE_F32
 
 inline int whole(int64_t n, int dt) { const int V = 16 / dtype_bytes(dt); return (int)((n + V - 1) / V * V); }      // up to whole 16-byte pieces
 
@@ -782,7 +793,7 @@ void pack_rows(const void* x, int64_t ld, int64_t rows, int cols, int dt, void* 
 hipError_t product(ProductArgs a, int dt, bool acol, bool bcol, bool packed, void* part, hipStream_t s) {
     const int V = 16 / dtype_bytes(dt);
     Plan p = plan_product(a.M, a.N, a.K, dt, acol, bcol);
-    a.vec = a.N % V == 0 && a.ldy % V == 0 && on16(a.y) && on16(a.bias) && (!a.res || (on16(a.res) && a.ldr % V == 0)) && on16(a.slope);
+    a.vec = a.N % V == 0 && a.ldy % V == 0 && on16(a.y) && on16(a.bias) && (!a.res || (on16(a.res) && a.ldr % V == 0)) && on(a.slope, V * (a.slope_f32 ? 4 : 2));
     // operands by 16-byte pieces: rows start on 16 bytes and whole pieces make up the contiguous axis
     const bool pieces = on16(a.A) && on16(a.B) && a.lda % V == 0 && a.ldb % V == 0 && (acol ? a.own_a % V == 0 : packed || a.K % V == 0) &&
                         (bcol ? a.own_b % V == 0 : packed || a.K % V == 0);
@@ -883,6 +894,8 @@ ADX_API int adx_op_linear_residual(const void* x, int64_t ldx, const void* w, in
                                    void* y, int64_t ldy, int64_t M, int N, int K, int act, int dtype, void* workspace, size_t workspace_bytes,
                                    void* stream) {
     if (!dtype_ok(dtype)) { set_error("linear_residual: unknown element type"); return ADX_EINVAL; }
+    const bool slope_f32 = (act & SLOPE_F32) || dtype == DT_F32;
+    act &= ~SLOPE_F32;
     if (act < ACT_NONE || act > ACT_TANH_) { set_error("linear_residual: unknown activation"); return ADX_EINVAL; }
     if (!shape_ok(M, N, K)) { set_error("linear_residual: needs 0 <= M <= 2^30 and 0 < N, K <= 2^26"); return ADX_EINVAL; }
     if (M == 0) return ADX_OK;
@@ -896,7 +909,7 @@ ADX_API int adx_op_linear_residual(const void* x, int64_t ldx, const void* w, in
     unsigned char* base = static_cast<unsigned char*>(workspace);
     ProductArgs a{};
     a.A = x; a.lda = ldx; a.B = w; a.ldb = ldw; a.M = M; a.N = N; a.K = K; a.bias = bias; a.res = res; a.ldr = ldr; a.slope = slope; a.y = y; a.ldy = ldy;
-    a.act = act;
+    a.act = act; a.slope_f32 = slope_f32;
     if (ws.pack) {
         pack_rows(x, ldx, M, K, dtype, base + ws.x, s);
         pack_rows(w, ldw, N, K, dtype, base + ws.w, s);
@@ -908,13 +921,15 @@ ADX_API int adx_op_linear_residual(const void* x, int64_t ldx, const void* w, in
 
 ADX_API size_t adx_linear_residual_bwd_ws_bytes(int64_t M, int N, int K, int act, int dtype) {
     if (!shape_ok(M, N, K) || !dtype_ok(dtype) || M == 0) return 0;
-    return bwd_workspace(M, N, K, act, dtype).bytes;
+    return bwd_workspace(M, N, K, act & ~SLOPE_F32, dtype).bytes;
 }
 
 ADX_API int adx_op_linear_residual_bwd(const void* dy, int64_t ldd, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* slope, void* dx,
                                        void* dw, void* db, int64_t M, int N, int K, int act, int dtype, void* workspace, size_t workspace_bytes,
                                        void* stream) {
     if (!dtype_ok(dtype)) { set_error("linear_residual_bwd: unknown element type"); return ADX_EINVAL; }
+    const bool slope_f32 = (act & SLOPE_F32) || dtype == DT_F32;
+    act &= ~SLOPE_F32;
     if (act < ACT_NONE || act > ACT_TANH_) { set_error("linear_residual_bwd: unknown activation"); return ADX_EINVAL; }
     if (!shape_ok(M, N, K) || M == 0) { set_error("linear_residual_bwd: needs 1 <= M <= 2^30 and 0 < N, K <= 2^26"); return ADX_EINVAL; }
     if (!dy || (dx && !w) || (dw && !x) || (act != ACT_NONE && !slope)) { set_error("linear_residual_bwd: null pointer"); return ADX_EINVAL; }
@@ -931,7 +946,7 @@ ADX_API int adx_op_linear_residual_bwd(const void* dy, int64_t ldd, const void* 
     const bool store = ws.store_dz && (dx || dw);
     const int Np = whole(N, dtype), Kp = whole(K, dtype);
     if (store || db) {
-        const bool vec = N % V == 0 && ldd % V == 0 && on16(dy) && on16(slope);
+        const bool vec = N % V == 0 && ldd % V == 0 && on16(dy) && on(slope, V * (slope_f32 ? 4 : 2));
         with_dtype(dtype, [&](auto t) {
             typedef decltype(t) T;
             const int cols = vec ? 64 * V : 64, width = store ? Np : N;
@@ -939,8 +954,13 @@ ADX_API int adx_op_linear_residual_bwd(const void* dy, int64_t ldd, const void* 
             void* to = store ? dz : nullptr;
             float* part = db ? sums : nullptr;
             void* whole_db = ws.chunks == 1 ? db : nullptr;
-            if (vec) hipLaunchKernelGGL((slope_kernel<T, true>), grid, dim3(256), 0, s, dy, ldd, slope, to, Np, part, whole_db, M, N, act);
-            else hipLaunchKernelGGL((slope_kernel<T, false>), grid, dim3(256), 0, s, dy, ldd, slope, to, Np, part, whole_db, M, N, act);
+            auto by_slope = [&](auto kept) {
+                typedef decltype(kept) S;
+                if (vec) hipLaunchKernelGGL((slope_kernel<T, S, true>), grid, dim3(256), 0, s, dy, ldd, slope, to, Np, part, whole_db, M, N, act);
+                else hipLaunchKernelGGL((slope_kernel<T, S, false>), grid, dim3(256), 0, s, dy, ldd, slope, to, Np, part, whole_db, M, N, act);
+            };
+            if (slope_f32) by_slope(float{});
+            else by_slope(typename Code<T>::type{});
             if (db && ws.chunks > 1) hipLaunchKernelGGL(colsum_join_kernel<T>, dim3((unsigned)((N + 63) / 64)), dim3(64 * JOIN_WAVES), 0, s, sums, ws.chunks, N, db);
         });
     }

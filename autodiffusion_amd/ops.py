@@ -368,11 +368,7 @@ def _on_pieces(t: torch.Tensor, ld: int):
     return t, ld
 
 
-def _linear_sizes(what: str, N: int, K: int, act: int) -> None:
-    if N > 1 << 26 or K > 1 << 26:
-        raise ValueError(f"{what}: widths of at most 2^26")
-    if not _lib.ACT_NONE <= act <= _lib.ACT_TANH:
-        raise ValueError(f"{what}: unknown activation {act}")
+_MOST_WIDE = 1 << 26
 
 
 @functools.lru_cache(maxsize=4096)
@@ -383,10 +379,12 @@ def _linear_residual_bytes(M: int, N: int, K: int, dt: int, act: int = -1) -> in
 
 @on_data_device
 def linear_residual(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
-                    act: int = _lib.ACT_NONE, keep_slope: bool = False):
+                    act: int = _lib.ACT_NONE, keep_slope=False):
     """``act(x w^T + bias) + residual`` in the tensors' own type (fp32, bf16 or fp16, all the same; fp32 sums, one rounding): x (..., K),
     w (N, K), bias (N,), residual (..., N).  ``act``: ACT_NONE .. ACT_TANH.  ``keep_slope`` also returns the activation's slope, which
-    ``linear_residual_bwd`` needs: fp32 for fp32 tensors, 16-bit codes (see adx.h) in an int16 tensor otherwise.  Rows of x, w and residual may be strided (adjacent values in a row)."""
+    ``linear_residual_bwd`` needs: with torch.float32 in fp32; with True fp32 for fp32 tensors and 16-bit codes (see adx.h) in an int16 tensor
+    otherwise -- exact for ACT_RELU and ACT_LEAKY, while slopes of the smooth activations below 2^-16 vanish.  Rows of x, w and residual may be
+    strided (adjacent values in a row)."""
     dtype = x.dtype
     dt = DTYPES.get(dtype)
     if dt is None or w.dtype != dtype or (bias is not None and bias.dtype != dtype) or (residual is not None and residual.dtype != dtype):
@@ -396,13 +394,17 @@ def linear_residual(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tenso
     N, K = w.shape
     if x.shape[-1] != K or N == 0 or K == 0:
         raise ValueError("linear_residual: x (..., K) and w (N, K)")
-    _linear_sizes("linear_residual", N, K, act)
+    if N > _MOST_WIDE or K > _MOST_WIDE or not 0 <= act <= _lib.ACT_TANH:
+        raise ValueError(f"linear_residual: widths {N} and {K} of at most 2^26, activation code {act} of ACT_NONE .. ACT_TANH")
+    wide = keep_slope is torch.float32
+    if keep_slope is not False and keep_slope is not True and not wide:
+        raise ValueError("linear_residual: keep_slope is False, True or torch.float32")
     out_shape = (*x.shape[:-1], N)
     if (bias is not None and bias.shape != (N,)) or (residual is not None and residual.shape != out_shape):
         raise ValueError("linear_residual: bias (N,) and residual of the output's shape")
     stream = stream_on(device_of("linear_residual", x, w, bias, residual))
     y = x.new_empty(out_shape)
-    slope = x.new_empty(out_shape, dtype=_SLOPE[dt]) if keep_slope else None
+    slope = x.new_empty(out_shape, dtype=keep_slope if wide else _SLOPE[dt]) if keep_slope else None
     x2, ldx = _rows(x)
     M = x2.shape[0]
     if M:
@@ -415,7 +417,7 @@ def linear_residual(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tenso
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         check(_lib.load().adx_op_linear_residual(x2.data_ptr(), ldx, w2.data_ptr(), ldw, None if b is None else b.data_ptr(),
                                                  None if r2 is None else r2.data_ptr(), ldr, None if slope is None else slope.data_ptr(), y.data_ptr(), N,
-                                                 M, N, K, act, dt, None if ws is None else ws.data_ptr(), need, stream), "linear_residual")
+                                                 M, N, K, act | _lib.SLOPE_F32 if wide else act, dt, None if ws is None else ws.data_ptr(), need, stream), "linear_residual")
     return (y, slope) if keep_slope else y
 
 
@@ -428,14 +430,16 @@ def linear_residual_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, slop
     dt = DTYPES.get(dtype)
     if dt is None or x.dtype != dtype or w.dtype != dtype:
         raise ValueError("linear_residual_bwd: dy, x and w are fp32, bf16 or fp16, all the same")
-    if slope is not None and slope.dtype != _SLOPE[dt]:
+    wide = slope is not None and slope.dtype == torch.float32
+    if slope is not None and not wide and slope.dtype != _SLOPE[dt]:
         raise ValueError("linear_residual_bwd: slope is what linear_residual returned with keep_slope")
     if w.dim() != 2 or x.dim() < 1:
         raise ValueError("linear_residual_bwd: x (..., K), w (N, K), dy and slope (..., N)")
     N, K = w.shape
     if x.shape[-1] != K or dy.shape != (*x.shape[:-1], N) or (slope is not None and slope.shape != dy.shape):
         raise ValueError("linear_residual_bwd: x (..., K), w (N, K), dy and slope (..., N)")
-    _linear_sizes("linear_residual_bwd", N, K, act)
+    if N > _MOST_WIDE or K > _MOST_WIDE or not 0 <= act <= _lib.ACT_TANH:
+        raise ValueError(f"linear_residual_bwd: widths {N} and {K} of at most 2^26, activation code {act} of ACT_NONE .. ACT_TANH")
     if act != _lib.ACT_NONE and slope is None:
         raise ValueError("linear_residual_bwd: the activation's gradient needs slope (linear_residual with keep_slope)")
     stream = stream_on(device_of("linear_residual_bwd", dy, x, w, slope))
@@ -455,6 +459,6 @@ def linear_residual_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, slop
         ws = torch.empty(need, dtype=torch.uint8, device=x.device)
         check(_lib.load().adx_op_linear_residual_bwd(g.data_ptr(), ldd, x2.data_ptr(), ldx, w2.data_ptr(), ldw, None if z is None else z.data_ptr(),
                                                      None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
-                                                     None if db is None else db.data_ptr(), M, N, K, act, dt, ws.data_ptr(), need, stream),
+                                                     None if db is None else db.data_ptr(), M, N, K, act | _lib.SLOPE_F32 if wide else act, dt, ws.data_ptr(), need, stream),
               "linear_residual_bwd")
     return dx, dw, db

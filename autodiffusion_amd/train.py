@@ -870,7 +870,8 @@ class _LinearResidual(torch.autograd.Function):
         grad = recorded and (need[0] or need[1] or need[2])
         slope = None
         if grad and act_code != _lib.ACT_NONE:
-            y, slope = ops.linear_residual(x, w, bias, residual, act_code, True)
+            # 16-bit codes hold the slopes of ReLU and LeakyReLU exactly, not the small ones of the others
+            y, slope = ops.linear_residual(x, w, bias, residual, act_code, act_code in (_lib.ACT_RELU, _lib.ACT_LEAKY) or torch.float32)
         else:
             y = ops.linear_residual(x, w, bias, residual, act_code)
         ctx.act_code = act_code
@@ -892,6 +893,6 @@ class _LinearResidual(torch.autograd.Function):
 def linear_residual(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
                     act: int = _lib.ACT_NONE) -> torch.Tensor:
     """``ops.linear_residual`` with gradients for x, w, bias and residual.  For the backward it keeps x, w and the
-    activation's slope (in 16 bits where the tensors have 16); without gradients nothing.  Forward-mode derivatives are refused, with gradients
+    activation's slope (fp32; 16 bits a value for ACT_RELU and ACT_LEAKY on 16-bit tensors); without gradients nothing.  Forward-mode derivatives are refused, with gradients
     enabled or not."""
     return _LinearResidual.apply(x, w, bias, residual, act, torch.is_grad_enabled())

@@ -49,6 +49,8 @@ enum { ADX_PREC_F32 = 0, ADX_PREC_BF16 = 1, ADX_PREC_BF16X3 = 2,
        ADX_PREC_F16 = 4 };
 /* Element types of the operators that take more than fp32 tensors. */
 enum { ADX_DT_F32 = 0, ADX_DT_BF16 = 1, ADX_DT_F16 = 2 };
+/* Or-ed to the activation of adx_op_linear_residual and its backward: the kept slope is fp32 for every element type. */
+enum { ADX_SLOPE_F32 = 0x100 };
 enum { ADX_VARIANT_A = 0, ADX_VARIANT_DIT = 1, ADX_VARIANT_MMDIT = 2 };
 
 /* sampling flags */
@@ -307,8 +309,9 @@ int adx_op_rope(const void* q, void* q_out, int heads_q, const void* k, void* k_
                 int B, int S, int dh, int rotary_dim, int interleaved, int inverse, int dtype, void* stream);
 /* y[M][N] = act(x[M][K] w[N][K]^T + bias[N]) + res[M][N], M <= 2^30, N and K <= 2^26; bias, res nullable; all tensors of one element
  * type, adjacent values in a row; row strides (elements) ldy >= N and ldx, ldw, ldr >= 0 (0: one row for all).  act: ADX_ACT_NONE .. ADX_ACT_TANH.  slope (nullable,
- * [M][N] contiguous) receives what the gradient needs for act != ADX_ACT_NONE, act' of the sum: fp32 values for fp32 tensors; for 16-bit
- * tensors uint16 codes q of (q - 8192) / 32768 (0: NaN; LeakyReLU's 8520 stands for 0.01 itself).
+ * [M][N] contiguous) receives what the gradient needs for act != ADX_ACT_NONE, act' of the sum: fp32 values for fp32 tensors and, with
+ * act | ADX_SLOPE_F32 (the same in the backward), for 16-bit ones; else for 16-bit tensors uint16 codes q of (q - 8192) / 32768 (0: NaN; LeakyReLU's 8520
+ * stands for 0.01 itself): exact for ReLU and LeakyReLU, to 2^-16 for the smooth activations -- smaller slopes (GELU below -4.5, tanh beyond 6) are lost.
  * y and slope overlap no input, except that y may be res itself (same pointer and stride).  M = 0 does nothing.
  * workspace: adx_linear_residual_ws_bytes(M, N, K, dtype) bytes, 16-byte aligned (0: may be NULL), the call's own until it has run. */
 size_t adx_linear_residual_ws_bytes(int64_t M, int N, int K, int dtype);

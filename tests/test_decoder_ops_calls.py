@@ -4,7 +4,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fw
 
-from autodiffusion_amd import ops, str_backbone, train
+from autodiffusion_amd import _lib, ops, str_backbone, train
 
 
 @pytest.fixture
@@ -88,3 +88,21 @@ def test_sizes_beyond_32_bits_are_refused():
     for bad in (dict(top_k=WRAP + 2), dict(top_k=2 - WRAP), dict(top_k=0), dict(top_k=9), dict(x=huge(WRAP + 4, 32, dtype=torch.float32))):
         with pytest.raises(ValueError, match="top_k"):
             str_backbone.moe_few(**(ok | bad))
+
+
+def test_forms_of_the_kept_slope():
+    x, w = torch.zeros(5, 16, dtype=torch.bfloat16), torch.zeros(8, 16, dtype=torch.bfloat16)
+    for keep in (torch.float16, torch.int16, "fp32", 1):
+        with pytest.raises(ValueError, match="keep_slope"):
+            ops.linear_residual(x, w, act=2, keep_slope=keep)
+    for slope in (torch.zeros(5, 8, dtype=torch.bfloat16), torch.zeros(5, 8, dtype=torch.float64), torch.zeros(5, 7)):
+        with pytest.raises(ValueError, match="slope"):
+            ops.linear_residual_bwd(torch.zeros(5, 8, dtype=torch.bfloat16), x, w, slope, act=2)
+    for slope in (torch.zeros(5, 8, dtype=torch.int16), torch.zeros(5, 8)):
+        with pytest.raises(_lib.AdxError, match="device memory"):
+            ops.linear_residual_bwd(torch.zeros(5, 8, dtype=torch.bfloat16), x, w, slope, act=2)
+    lib, pointer = _lib.load(), 4096                     # refused before it is used
+    assert lib.adx_linear_residual_bwd_ws_bytes(100, 64, 64, 2 | _lib.SLOPE_F32, 1) == lib.adx_linear_residual_bwd_ws_bytes(100, 64, 64, 2, 1)
+    for act in (7, -1):
+        assert lib.adx_op_linear_residual(pointer, 64, pointer, 64, None, None, 0, None, pointer, 64, 100, 64, 64, act | _lib.SLOPE_F32, 1, None, 0, None) == 1
+        assert b"activation" in lib.adx_last_error()
