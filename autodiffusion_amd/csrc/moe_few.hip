@@ -535,7 +535,7 @@ __global__ __launch_bounds__(64 * WAVES, P == P_F32 || (P == P_BF16 && sizeof(A)
         for (int j = 0; j < J; ++j) {
             const int i = min(i0 + j * 64 * WAVES, items - 1);
             t[j] = i / (COLS / 2);
-            c[j] = min(col0 + i % (COLS / 2) * 2, a.d - 2);               // columns behind d repeat the last two
+            c[j] = min(col0 + i % (COLS / 2) * 2, a.d - 2);               // columns behind d load the last two again
             s0[j] = s1[j] = 0.f;
         }
         for (int q0 = 0; q0 < terms; q0 += C) {
@@ -562,7 +562,9 @@ __global__ __launch_bounds__(64 * WAVES, P == P_F32 || (P == P_BF16 && sizeof(A)
         }
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            if (i0 + j * 64 * WAVES >= items) break;
+            const int i = i0 + j * 64 * WAVES;
+            if (i >= items) break;
+            if (col0 + i % (COLS / 2) * 2 >= a.d) continue;               // stored once: y may be the residual
             const int64_t at = (int64_t)t[j] * a.d + c[j];
             Pack<A, 2> r, o;
             if (res) r = *reinterpret_cast<const Pack<A, 2>*>(res + at);

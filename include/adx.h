@@ -327,7 +327,7 @@ int adx_op_linear_residual_bwd(const void* dy, int64_t ldd, const void* x, int64
 /* adx_op_moe_block for a few tokens (1 <= T <= 64; d, inter multiples of 32, d * inter <= 2^28; E <= 64, top_k <= 8): the same expert layer in two kernels (three where the
  * routing is large) that read the chosen experts' weights once.  x, res (nullable), y: [T][d] of act_type; router_w [E][d] fp32; w13, w2 as
  * for adx_op_moe_block under `precision`: fp32 tokens with ADX_PREC_F32, BF16, BF16X3 or F16 (fp16 bits) weights, bf16 tokens with
- * ADX_PREC_BF16, fp16 tokens with ADX_PREC_F16.  Tokens and hidden values are not rounded below their fp32 accuracy (16-bit act_type:
+ * ADX_PREC_BF16, fp16 tokens with ADX_PREC_F16.  y may be res itself and overlaps no other input.  Tokens and hidden values are not rounded below their fp32 accuracy (16-bit act_type:
  * 2^-16).  The routing is that of adx_op_moe_block and is left at the head of the workspace the same way (T * top_k int32, then
  * from the next multiple of 256 bytes T * top_k floats); a token whose router probabilities are NaN goes to the first experts.
  * workspace: adx_moe_few_workspace_bytes bytes, 16-byte aligned, contents arbitrary, the call's own until it has run.  No host

@@ -88,3 +88,20 @@ def test_gradients_of_saturated_units(dev, kind, act):
     within(dx, dz @ w.double(), e @ aw + (N + 2) * U24 * (dz.abs() + e) @ aw, kind, "dx")
     if kind != "fp16" and act in ("silu", "gelu_erf"):
         assert (db.float().abs()[: N // 2] > 0).all()               # small, not nothing
+
+
+# ---------------------------------------------------------------------------------------------------------------- expert layer
+@pytest.mark.parametrize("kind,precision,T,d", [("bf16", "bf16", 40, 160), ("fp32", "fp32", 64, 96), ("fp32", "bf16x3", 17, 32), ("fp16", "f16", 3, 96)])
+def test_moe_few_onto_the_residual(dev, kind, precision, T, d):
+    """The raw entry with y in place of the residual, widths that end inside a group of 64 output columns: the bits of the call beside it."""
+    from autodiffusion_amd import _lib, str_backbone
+    g = torch.Generator().manual_seed(T + d)
+    x, res, router = rand(g, T, d, kind=kind), rand(g, T, d, kind=kind), rand(g, 8, d, scale=d ** -0.5)
+    s13, s2, _, _ = few_weights(g, 8, d, 96, precision)
+    want = str_backbone.moe_few(x, res, router, s13, s2, 96, 8, 2, precision)
+    lib, dt, prec = _lib.load(), _lib.DTYPES[TYPES[kind]], _lib.PRECISIONS[precision]
+    need = lib.adx_moe_few_workspace_bytes(T, d, 96, 8, 2, dt, prec)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _lib.check(lib.adx_op_moe_few(x.data_ptr(), res.data_ptr(), router.data_ptr(), s13.data_ptr(), s2.data_ptr(), T, d, 96, 8, 2, dt, prec, ws.data_ptr(),
+                                  need, res.data_ptr(), torch.cuda.current_stream().cuda_stream), "moe_few")
+    assert torch.equal(res, want)
