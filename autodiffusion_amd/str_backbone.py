@@ -92,6 +92,10 @@ def prepare_expert_weights(w1: List[torch.Tensor], w3: List[torch.Tensor], w2: L
 _FEW_WEIGHTS = {"fp32": (torch.float32,), "bf16": (torch.bfloat16, torch.int16), "bf16x3": (torch.int16, torch.bfloat16), "f16": (torch.float16, torch.int16)}
 
 
+def _on16(t: torch.Tensor) -> torch.Tensor:
+    return t.clone() if t.data_ptr() % 16 else t
+
+
 @functools.lru_cache(maxsize=4096)
 def _moe_few_bytes(T: int, d: int, inter: int, n_experts: int, top_k: int, dt: int, prec: int) -> int:
     return int(_lib.load().adx_moe_few_workspace_bytes(T, d, inter, n_experts, top_k, dt, prec))
@@ -102,7 +106,7 @@ def moe_few(x: torch.Tensor, res: Optional[torch.Tensor], router_w: torch.Tensor
             top_k: int, precision: str = "fp32", workspace: Optional[torch.Tensor] = None, return_routing: bool = False):
     """``moe_block`` for at most 64 tokens in two kernels.  x, res (T, d) fp32 with weights of any ``precision`` ("fp32" | "bf16" | "bf16x3" |
     "f16"), or bf16 with "bf16", or fp16 with "f16" weights; returns x's type.  w13 / w2: as ``prepare_expert_weights`` returns them, or the
-    plain (E, 2 inter, d) / (E, d, inter) tensors of that type.  router_w (E, d) fp32."""
+    plain (E, 2 inter, d) / (E, d, inter) tensors of that type, starting on 16 bytes.  router_w (E, d) fp32."""
     dtype = x.dtype
     dt, prec, kinds = DTYPES.get(dtype), _lib.PRECISIONS[precision], _FEW_WEIGHTS.get(precision)
     if dt is None or x.dim() != 2 or (res is not None and (res.dtype != dtype or res.shape != x.shape)):
@@ -124,10 +128,10 @@ def moe_few(x: torch.Tensor, res: Optional[torch.Tensor], router_w: torch.Tensor
     if T == 0:
         none = x.new_empty((0, top_k), dtype=torch.float32)
         return (y, none.int(), none) if return_routing else y
-    x, router_w = x.contiguous(), router_w.contiguous()
-    res = None if res is None else res.contiguous()
+    x, router_w = _on16(x.contiguous()), _on16(router_w.contiguous())
+    res = None if res is None else _on16(res.contiguous())
     need = _moe_few_bytes(T, d, inter, n_experts, top_k, dt, prec)
-    if workspace is None or workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
+    if workspace is None or workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous() or workspace.data_ptr() % 16:
         workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
     check(_lib.load().adx_op_moe_few(x.data_ptr(), None if res is None else res.data_ptr(), router_w.data_ptr(), w13.data_ptr(), w2.data_ptr(), T, d, inter,
                                      n_experts, top_k, dt, prec, workspace.data_ptr(), workspace.numel() * workspace.element_size(), y.data_ptr(), stream),

@@ -105,3 +105,25 @@ def test_moe_few_onto_the_residual(dev, kind, precision, T, d):
     _lib.check(lib.adx_op_moe_few(x.data_ptr(), res.data_ptr(), router.data_ptr(), s13.data_ptr(), s2.data_ptr(), T, d, 96, 8, 2, dt, prec, ws.data_ptr(),
                                   need, res.data_ptr(), torch.cuda.current_stream().cuda_stream), "moe_few")
     assert torch.equal(res, want)
+
+
+def test_moe_few_of_tensors_that_start_anywhere(dev):
+    """Tokens, residual, router and workspace behind a few values of another tensor: the bits of the call on tensors of their own.  Weights off 16
+    bytes are refused, not copied on every call."""
+    from autodiffusion_amd import _lib, str_backbone
+    g = torch.Generator().manual_seed(41)
+
+    def shifted(t, by):
+        flat = torch.zeros(t.numel() + by, dtype=t.dtype, device=dev)
+        flat[by:] = t.flatten()
+        return flat[by:].view(t.shape)
+
+    for kind, precision in (("bf16", "bf16"), ("fp32", "fp32"), ("fp32", "bf16x3")):
+        x, res, router = rand(g, 5, 64, kind=kind), rand(g, 5, 64, kind=kind), rand(g, 8, 64)
+        s13, s2, _, _ = few_weights(g, 8, 64, 96, precision)
+        want = str_backbone.moe_few(x, res, router, s13, s2, 96, 8, 2, precision)
+        ws = torch.empty(1 << 22, dtype=torch.uint8, device=dev)[1:]
+        for by in (1, 3):
+            assert torch.equal(str_backbone.moe_few(shifted(x, by), shifted(res, by), shifted(router, by), s13, s2, 96, 8, 2, precision, workspace=ws), want)
+        with pytest.raises(_lib.AdxError, match="aligned"):
+            str_backbone.moe_few(x, res, router, shifted(s13, 1), s2, 96, 8, 2, precision)
