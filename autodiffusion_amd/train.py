@@ -827,9 +827,27 @@ def _first_order(what: str) -> None:
         raise RuntimeError(f"{what}: gradients of gradients are not built")
 
 
+_Accumulator = torch._C._functions.AccumulateGrad
+
+
+def _leaves_on(ctx, what: str, stream: int, capturing) -> None:
+    """The gradient of a leaf is accumulated on the stream of the pass that first reached it, as long as a graph of that pass lives; a capture that
+    is led to another stream ends the process.  Every recorded pass leaves its stream with the accumulators of its leaves, and a
+    capture that finds another one there is refused (passes that reach a leaf by other operators alone leave nothing)."""
+    for node, _ in ctx.next_functions:
+        if type(node) is _Accumulator and node.metadata.setdefault("adx_stream", stream) != stream and capturing():
+            raise RuntimeError(f"{what}: captured while a graph of an earlier pass over the same leaves is alive: drop its outputs and losses first")
+
+
+def _leaves_on_current(ctx, what: str, device: int) -> None:
+    if device >= 0:
+        _leaves_on(ctx, what, torch._C._cuda_getCurrentRawStream(device), torch.cuda.is_current_stream_capturing)
+
+
 class _Rope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, amplitude, layout):
+        _leaves_on_current(ctx, "rope", q.get_device())
         ctx.set_materialize_grads(False)
         at_tensor = isinstance(positions, torch.Tensor)
         ctx.save_for_backward(positions if at_tensor else None, inv_freq)
@@ -866,6 +884,7 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions, inv_freq: torch.
 class _LinearResidual(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, act_code, recorded):
+        _leaves_on_current(ctx, "linear_residual", x.get_device())
         need = ctx.needs_input_grad                      # what the inputs want, also where no graph is recorded
         grad = recorded and (need[0] or need[1] or need[2])
         slope = None

@@ -106,3 +106,33 @@ def test_forms_of_the_kept_slope():
     for act in (7, -1):
         assert lib.adx_op_linear_residual(pointer, 64, pointer, 64, None, None, 0, None, pointer, 64, 100, 64, 64, act | _lib.SLOPE_F32, 1, None, 0, None) == 1
         assert b"activation" in lib.adx_last_error()
+
+
+def test_capture_over_the_leaves_of_a_live_graph_is_refused():
+    """On made-up streams: a pass on one stream, then captures on another while its graph lives and after."""
+    class Scaled(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, stream, capturing):
+            train._leaves_on(ctx, "scaled", stream, lambda: capturing)
+            return 2 * x
+
+        @staticmethod
+        def backward(ctx, dy):
+            return 2 * dy, None, None
+
+    w = torch.randn(3, requires_grad=True)
+    y = Scaled.apply(w, 1, False)
+    Scaled.apply(w, 1, True)                                         # the same stream
+    z = Scaled.apply(w, 2, False)                                    # eager passes on any stream
+    with pytest.raises(RuntimeError, match="earlier pass"):
+        Scaled.apply(w, 2, True)
+    del y
+    with pytest.raises(RuntimeError, match="earlier pass"):          # the accumulator is still the first pass's
+        Scaled.apply(w, 2, True)
+    assert torch.equal(torch.autograd.grad(z.sum(), w)[0], torch.full((3,), 2.0))
+    del z
+    y = Scaled.apply(w, 2, True)
+    z = Scaled.apply(w * 1, 2, True) + Scaled.apply(w, 2, True)      # further passes of the same capture, not only over leaves
+    assert torch.equal(torch.autograd.grad((y + z).sum(), w)[0], torch.full((3,), 6.0))
+    with torch.no_grad():
+        Scaled.apply(w, 3, True)                                     # nothing is recorded

@@ -127,3 +127,35 @@ def test_moe_few_of_tensors_that_start_anywhere(dev):
             assert torch.equal(str_backbone.moe_few(shifted(x, by), shifted(res, by), shifted(router, by), s13, s2, 96, 8, 2, precision, workspace=ws), want)
         with pytest.raises(_lib.AdxError, match="aligned"):
             str_backbone.moe_few(x, res, router, shifted(s13, 1), s2, 96, 8, 2, precision)
+
+
+# ---------------------------------------------------------------------------------------------------------------- captures
+def test_capture_beside_a_live_eager_graph_is_refused(dev):
+    """Capturing a step over leaves of an eager graph that is still alive raises, and the program goes on: the eager graph's gradients, then the
+    capture, once that graph is gone."""
+    from autodiffusion_amd import ops, train
+    g = torch.Generator().manual_seed(51)
+    freq, amp = ops.rope_frequencies(16)
+    x, w, dy = rand(g, 70, 64), rand(g, 64, 64, scale=1 / 8).requires_grad_(), rand(g, 70, 64)
+    q, dq = rand(g, 1, 5, 4, 16).requires_grad_(), rand(g, 1, 5, 4, 16)
+    forms = ((lambda: train.linear_residual(x, w, act=2), w, dy), (lambda: train.rope(q, None, 3, freq, amp)[0], q, dq))
+    for forward, leaf, up in forms:
+        want = torch.autograd.grad(forward(), leaf, up)[0].clone()
+        alive = forward()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="earlier pass"):
+            with torch.cuda.graph(graph):
+                forward()
+        assert torch.equal(torch.autograd.grad(alive, leaf, up)[0], want)
+        del alive
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(forward(), leaf, up)[0]
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+            forward()
