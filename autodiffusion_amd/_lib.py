@@ -40,6 +40,7 @@ EXPORTS = [
     "adx_op_dropout", "adx_op_attention_stats_dropout", "adx_op_attention_bwd_dropout", "adx_op_attention_dropout_mask",
     "adx_op_rmsnorm", "adx_op_rotary", "adx_moe_workspace_bytes", "adx_op_moe_block",
     "adx_op_rope", "adx_op_linear_residual", "adx_linear_residual_ws_bytes", "adx_op_linear_residual_bwd", "adx_linear_residual_bwd_ws_bytes",
+    "adx_linear_residual_edge",
     "adx_op_moe_few", "adx_moe_few_workspace_bytes",
 ]
 
@@ -147,6 +148,7 @@ def load() -> C.CDLL:
         "adx_op_linear_residual": ([p, i64, p, i64, p, p, i64, p, p, i64, i64, i, i, i, i, p, C.c_size_t, p], i),
         "adx_linear_residual_ws_bytes": ([i64, i, i, i], C.c_size_t),
         "adx_op_linear_residual_bwd": ([p, i64, p, i64, p, i64, p, p, p, p, i64, i, i, i, i, p, C.c_size_t, p], i),
+        "adx_linear_residual_edge": ([i64, i, i, i, i], i),
         "adx_linear_residual_bwd_ws_bytes": ([i64, i, i, i, i], C.c_size_t),
         "adx_op_moe_few": ([p, p, p, p, p, i, i, i, i, i, i, i, p, C.c_size_t, p, p], i),
         "adx_moe_few_workspace_bytes": ([i, i, i, i, i, i, i], C.c_size_t),

@@ -885,6 +885,13 @@ using namespace adx;
 
 #define ADX_API extern "C" __attribute__((visibility("default")))
 
+ADX_API int adx_linear_residual_edge(int64_t M, int N, int K, int which, int dtype) {
+    if (!shape_ok(M, N, K) || M == 0 || !dtype_ok(dtype)) return -1;
+    if (which == 0) return plan_product(M, N, K, dtype, false, false).tile;
+    if (which == 1) return plan_product(M, K, N, dtype, false, true).tile;
+    return which == 2 ? plan_product(N, K, M, dtype, true, true).tile : -1;
+}
+
 ADX_API size_t adx_linear_residual_ws_bytes(int64_t M, int N, int K, int dtype) {
     if (!shape_ok(M, N, K) || !dtype_ok(dtype) || M == 0) return 0;
     return fwd_workspace(M, N, K, dtype).bytes;

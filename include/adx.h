@@ -317,6 +317,9 @@ int adx_op_rope(const void* q, void* q_out, int heads_q, const void* k, void* k_
 size_t adx_linear_residual_ws_bytes(int64_t M, int N, int K, int dtype);
 int adx_op_linear_residual(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldr, void* slope,
                            void* y, int64_t ldy, int64_t M, int N, int K, int act, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+/* Edge of the square tiles that y (which = 0), dx (1) or dw (2) of that size is computed in -- 64, 128 or 256, 0: no tiles (few rows) -- where rows start
+ * on 16 bytes or are laid out anew; -1: sizes that are refused. */
+int adx_linear_residual_edge(int64_t M, int N, int K, int which, int dtype);
 /* Its gradients, any of them NULL where not wanted: with dz = dy slope, dx[M][K] = dz w, dw[N][K] = dz^T x, db[N] = column sums of
  * dz (the residual's gradient is dy itself).  slope may be NULL for ADX_ACT_NONE.  dz is rounded to the element type as the operand of the two
  * products; db sums the unrounded values.  Sums over rows are joined in a fixed order (no atomics): bit-identical re-runs. */

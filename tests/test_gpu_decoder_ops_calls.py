@@ -76,18 +76,186 @@ def test_gradients_of_saturated_units(dev, kind, act):
     assert kept.dtype == (torch.int16 if act in ("relu", "leaky") and kind != "fp32" else torch.float32)
     dx, dw, db = torch.autograd.grad(y, leaves, dy)
     x, w, b = (t.detach() for t in leaves)
+    gradients_within(kind, act, x, w, b, dy, (dx, dw, db))
+    if kind != "fp16" and act in ("silu", "gelu_erf"):
+        assert (db.float().abs()[: N // 2] > 0).all()               # small, not nothing
+
+
+# ---------------------------------------------------------------------------------------------------------------- every tile of the product
+def edges(M, N, K, kind):
+    """Edges of the tiles that y, dx and dw are computed in."""
+    from autodiffusion_amd import _lib
+    return tuple(_lib.load().adx_linear_residual_edge(M, N, K, which, _lib.DTYPES[TYPES[kind]]) for which in range(3))
+
+
+def gradients_within(kind, act, x, w, b, dy, got, what=""):
+    """(dx, dw, db) of the product with its slopes in fp32, elementwise."""
+    (M, K), N = x.shape, w.shape[0]
     _, _, z, ez = linear_exact(x, w, b, None, "none")
     d = slope_tails(z, act)
     moved = torch.maximum((slope_tails(z + ez, act) - d).abs(), (slope_tails(z - ez, act) - d).abs())         # what the rounding of z changes
     dz = dy.double() * d
-    ed = dy.double().abs() * (slope_error(z, act) + moved) + U24 * dz.abs()                            # as a summand
-    e = ed + HALF_STEP[kind] * dz.abs() + TINY[kind]                                                   # as an operand
-    ax, aw = x.double().abs(), w.double().abs()
-    within(db, dz.sum(0), ed.sum(0) + (M + 2) * U24 * (dz.abs() + ed).sum(0), kind, "db")
-    within(dw, dz.t() @ x.double(), e.t() @ ax + (M + 2) * U24 * (dz.abs() + e).t() @ ax, kind, "dw")
-    within(dx, dz @ w.double(), e @ aw + (N + 2) * U24 * (dz.abs() + e) @ aw, kind, "dx")
-    if kind != "fp16" and act in ("silu", "gelu_erf"):
-        assert (db.float().abs()[: N // 2] > 0).all()               # small, not nothing
+    ed = 0 * dz if act == "none" else dy.double().abs() * (slope_error(z, act) + moved) + U24 * dz.abs()       # as a summand
+    e = ed if act == "none" else ed + HALF_STEP[kind] * dz.abs() + TINY[kind]                                  # as an operand
+    ax, aw, ad = x.double().abs(), w.double().abs(), dz.abs() + e
+    within(got[0], dz @ w.double(), e @ aw + (N + 2) * U24 * ad @ aw, kind, f"{what} dx")
+    within(got[1], dz.t() @ x.double(), e.t().contiguous() @ ax + (M + 2) * U24 * ad.t().contiguous() @ ax, kind, f"{what} dw")
+    within(got[2], dz.sum(0), ed.sum(0) + (M + 2) * U24 * (dz.abs() + ed).sum(0), kind, f"{what} db")
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("M,N,K,edge", [(3590, 3608, 3624, 256), (2500, 2608, 2584, 128), (515, 520, 1032, 64)])
+def test_tiles_of_the_training_step(dev, kind, M, N, K, edge):
+    """y, dx and dw in tiles of each edge, ragged at both ends and in the summed axis, with an activation."""
+    from autodiffusion_amd import train
+    assert edges(M, N, K, kind) == (edge,) * 3
+    g = torch.Generator().manual_seed(M)
+    x, w, b, res, dy = (rand(g, *s, kind=kind, scale=c) for s, c in (((M, K), 1), ((N, K), K ** -0.5), ((N,), 1), ((M, N), 1), ((M, N), 1)))
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = train.linear_residual(*leaves, res, act=2)
+    got = torch.autograd.grad(y, leaves, dy)
+    x, w, b = (t.detach() for t in leaves)
+    want, e, _, _ = linear_exact(x, w, b, res, "gelu_erf")
+    within(y.detach(), want, e, kind, "y")
+    gradients_within(kind, "gelu_erf", x, w, b, dy, got)
+
+
+@pytest.mark.parametrize("kind,M,N,K,edge", [("fp32", 3590, 3604, 52, 256), ("fp32", 2600, 2500, 44, 128), ("fp16", 3590, 3608, 72, 256), ("fp16", 2600, 2504, 72, 128),
+                                             ("bf16", 2600, 2504, 72, 128)])
+def test_tiles_of_the_forward(dev, kind, M, N, K, edge):
+    """Large tiles over a few steps of the summed axis, with residual, bias and fp32 slopes."""
+    from autodiffusion_amd import ops
+    assert edges(M, N, K, kind)[0] == edge
+    g = torch.Generator().manual_seed(N)
+    x, w, b, res = rand(g, M, K, kind=kind), rand(g, N, K, kind=kind, scale=K ** -0.5), rand(g, N, kind=kind), rand(g, M, N, kind=kind)
+    y, slope = ops.linear_residual(x, w, b, res, act=5, keep_slope=torch.float32)
+    want, e, z, ez = linear_exact(x, w, b, res, "silu")
+    within(y, want, e, kind, "y")
+    assert bool(((slope.double() - slope_tails(z, "silu")).abs() <= 0.51 * ez + slope_error(z, "silu")).all())          # the slope changes by at most 1 / 2 a unit
+
+
+@pytest.mark.parametrize("kind,act,M,N,K", [("bf16", "gelu_erf", 1500, 1003, 501), ("fp16", "silu", 700, 999, 1101), ("fp32", "tanh", 900, 1021, 771),
+                                            ("bf16", "gelu_tanh", 1030, 515, 1001)])
+def test_training_step_laid_out_anew(dev, kind, act, M, N, K):
+    """Rows of no whole number of 16-byte pieces in a long product: operands and dz laid out anew, with an activation."""
+    from autodiffusion_amd import train
+    assert M * N * K >= 2 ** 28 and N % 4 and K % 4
+    g = torch.Generator().manual_seed(N)
+    leaves = [rand(g, *s, kind=kind, scale=c).requires_grad_() for s, c in (((M, K), 1), ((N, K), K ** -0.5), ((N,), 1))]
+    dy = rand(g, M, N, kind=kind)
+    y = train.linear_residual(*leaves, act=ACTS.index(act))
+    got = torch.autograd.grad(y, leaves, dy)
+    x, w, b = (t.detach() for t in leaves)
+    want, e, _, _ = linear_exact(x, w, b, None, act)
+    within(y.detach(), want, e, kind, "y")
+    gradients_within(kind, act, x, w, b, dy, got)
+
+
+def test_slopes_of_every_path(dev):
+    """fp32 slopes of 16-bit tensors from the few-row kernel, unaligned rows, a split sum and odd widths; the gradients from them."""
+    from autodiffusion_amd import ops
+    g = torch.Generator().manual_seed(32)
+    for kind in ("bf16", "fp16"):
+        for M, N, K in ((1, 8, 8), (17, 100, 36), (64, 130, 257), (130, 72, 40), (200, 257, 129), (70, 64, 4096), (129, 127, 2050)):
+            x, w, b, dy = rand(g, M, K, kind=kind), rand(g, N, K, kind=kind, scale=K ** -0.5), rand(g, N, kind=kind), rand(g, M, N, kind=kind)
+            for i, act in enumerate(ACTS):
+                if act in ("relu", "leaky"):                     # jump where the sum's sign is open
+                    continue
+                y, slope = ops.linear_residual(x, w, b, act=i, keep_slope=torch.float32)
+                assert torch.equal(y, ops.linear_residual(x, w, b, act=i))
+                _, _, z, ez = linear_exact(x, w, b, None, "none")
+                moved = torch.maximum((slope_tails(z + ez, act) - slope_tails(z, act)).abs(), (slope_tails(z - ez, act) - slope_tails(z, act)).abs())
+                assert bool(((slope.double() - slope_tails(z, act)).abs() <= slope_error(z, act) + moved).all()), act
+                got = ops.linear_residual_bwd(dy, x, w, slope, act=i)
+                gradients_within(kind, act, x, w, b, dy, got, act)
+                shifted = torch.empty(M * N + 1, device=dev)[1:].view(M, N).copy_(slope)             # slopes that start on 4 bytes
+                assert all(torch.equal(p, q) for p, q in zip(ops.linear_residual_bwd(dy, x, w, shifted, act=i), got))
+
+
+# ---------------------------------------------------------------------------------------------------------------- strides of the gradient's operands
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_gradient_of_strided_operands(dev, kind):
+    """x, w, dy and slopes as slices, transposed storage, leading axes and one row for all: the bits of the contiguous call; rows that start on
+    no 16 bytes: the formula."""
+    from autodiffusion_amd import ops
+    g = torch.Generator().manual_seed(33)
+    for M in (5, 200):
+        x, w, dy = rand(g, M, 200, kind=kind)[:, 8:168], rand(g, 96, 176, kind=kind, scale=0.1)[:, 16:], rand(g, M, 112, kind=kind)[:, 16:]
+        _, slope = ops.linear_residual(x, w, act=5, keep_slope=torch.float32)
+        want = ops.linear_residual_bwd(dy.contiguous(), x.contiguous(), w.contiguous(), slope, act=5)
+        gradients_within(kind, "silu", x, w, None, dy, want)
+        turned = [t.t().contiguous().t() for t in (dy, x, w, slope)]
+        wide = torch.empty(M, 100, device=dev)
+        wide[:, 3:99] = slope
+        deep = [t.reshape(M // 5, 5, -1) for t in (dy, x)]
+        for got in (ops.linear_residual_bwd(dy, x, w, slope, act=5), ops.linear_residual_bwd(*turned, act=5),
+                    ops.linear_residual_bwd(dy, x, w, wide[:, 3:99], act=5), ops.linear_residual_bwd(*deep, w, slope.reshape(M // 5, 5, 96), act=5)):
+            assert torch.equal(got[0].reshape(M, 160), want[0]) and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+        row = dy[:1].expand(M, 96)                                                          # one row for all
+        want = ops.linear_residual_bwd(row.contiguous(), x, w, slope, act=5)
+        assert all(torch.equal(p, q) for p, q in zip(ops.linear_residual_bwd(row, x, w, slope, act=5), want))
+        want = ops.linear_residual_bwd(dy, x[:1].expand(M, 160).contiguous(), w, slope, act=5)
+        assert all(torch.equal(p, q) for p, q in zip(ops.linear_residual_bwd(dy, x[:1].expand(M, 160), w, slope, act=5), want))
+        odd = [rand(g, t.shape[0], t.shape[1] + 1, kind=kind) for t in (dy, x, w)]
+        for o, t in zip(odd, (dy, x, w)):
+            o[:, 1:] = t
+        odd = [o[:, 1:] for o in odd]
+        gradients_within(kind, "silu", x, w, None, dy, ops.linear_residual_bwd(*odd, slope, act=5), "odd start")
+        gradients_within(kind, "silu", x[:, :-3], w[:, :-3], None, dy, ops.linear_residual_bwd(odd[0], odd[1][:, :-3], odd[2][:, :-3],
+                         ops.linear_residual(x[:, :-3], w[:, :-3], act=5, keep_slope=torch.float32)[1], act=5), "odd width")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+def test_rows_far_apart(dev, kind):
+    """Row strides of 2^21 values and more, whose tiles span more than 32 bits of bytes: forward and gradients."""
+    from autodiffusion_amd import ops
+    g = torch.Generator().manual_seed(34)
+    M, N, K, far = 80, 72, 96, (1 << 21) + 8
+
+    def spread(t):
+        flat = torch.empty((t.shape[0] - 1) * far + t.shape[1], dtype=t.dtype, device=dev)
+        out = flat.as_strided(t.shape, (far, 1))
+        out.copy_(t)
+        return out
+
+    x, w, dy, res = rand(g, M, K, kind=kind), rand(g, N, K, kind=kind, scale=0.1), rand(g, M, N, kind=kind), rand(g, M, N, kind=kind)
+    want, e, _, _ = linear_exact(x, w, None, res, "silu")
+    for a, b in ((spread(x), w), (x, spread(w)), (spread(x), spread(w))):
+        y, slope = ops.linear_residual(a, b, None, spread(res), act=5, keep_slope=torch.float32)
+        within(y, want, e, kind, "y")
+        gradients_within(kind, "silu", x, w, None, dy, ops.linear_residual_bwd(spread(dy), a, b, slope, act=5))
+    within(ops.linear_residual(spread(x)[:9], spread(w), None, res[:9], act=5), want[:9], e[:9], kind, "few rows")
+    plain = ops.linear_residual_bwd(spread(dy), x, w)                                       # dy itself is the operand
+    gradients_within(kind, "none", x, w, None, dy, plain)
+
+
+# ---------------------------------------------------------------------------------------------------------------- arguments that are not finite, or huge
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("M,N", [(5, 16), (80, 16), (70, 11)])
+def test_activations_of_extreme_arguments(dev, kind, M, N):
+    """What every activation and its slope give for infinities, NaN and the largest finite arguments (as biases of a product of zeros).  silu and the
+    gelus are z times a number that is 0 at -inf: NaN, as the formula says."""
+    from autodiffusion_amd import ops
+    inf, nan = math.inf, math.nan
+    top = [1e4, 6e4] if kind == "fp16" else [1e4, 1e18, 1e19, 1e30, 3e38]
+    z = torch.tensor(([inf, -inf, nan] + top + [-t for t in top] + [0.0] * 16)[:N]).to(TYPES[kind]).cuda()
+    x, w = torch.zeros(M, 24, dtype=TYPES[kind], device=dev), torch.zeros(N, 24, dtype=TYPES[kind], device=dev)
+    up, zero, one = torch.where(z > 0, z, 0 * z.abs().nan_to_num()), torch.zeros_like(z), torch.ones_like(z)
+    step, sign = (z > 0).to(z.dtype), torch.sign(z)
+    lowest = torch.where(z == -inf, z * 0, up)                     # NaN at -inf
+    known = torch.where(z.isinf(), z * 0, step)                    # slopes of 1 and 0, NaN at the infinities
+    known = torch.where(z == 0, 0.5 * one, known)
+    half = torch.where(z == 0, 0.5 * one, step)
+    expected = {"none": (z, one), "relu": (up, step), "leaky": (torch.where(z > 0, z, (z.double() * 0.01).to(z.dtype)), torch.where(z > 0, one.float(), 0.01)),
+                "silu": (lowest, known), "gelu_erf": (lowest, known), "gelu_tanh": (lowest, half), "tanh": (sign, torch.where(z == 0, one, zero))}
+    for i, act in enumerate(ACTS):
+        y, slope = ops.linear_residual(x, w, z, act=i, keep_slope=torch.float32)
+        value, d = (torch.where(z.isnan(), z, t.to(z.dtype)) if act != "none" else t for t in expected[act])
+        for m in (0, M - 1):
+            assert torch.allclose(y[m].double(), value.double(), rtol=2 * HALF_STEP[kind], atol=0, equal_nan=True), (act, y[m], value)
+            if act != "none":
+                d32 = torch.where(z.isnan(), nan, expected[act][1].float())
+                assert torch.allclose(slope[m], d32, rtol=60 * U24, atol=0, equal_nan=True), (act, slope[m], d32)
 
 
 # ---------------------------------------------------------------------------------------------------------------- expert layer
@@ -130,6 +298,7 @@ def test_moe_few_of_tensors_that_start_anywhere(dev):
 
 
 # ---------------------------------------------------------------------------------------------------------------- captures
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
 def test_capture_beside_a_live_eager_graph_is_refused(dev):
     """Capturing a step over leaves of an eager graph that is still alive raises, and the program goes on: the eager graph's gradients, then the
     capture, once that graph is gone."""
@@ -159,3 +328,37 @@ def test_capture_beside_a_live_eager_graph_is_refused(dev):
             torch.cuda.synchronize()
             assert torch.equal(got, want)
             forward()
+
+
+def test_few_token_layer_of_a_bf16_model(dev, monkeypatch):
+    """MixtralModel with few_token_experts under "bf16": its short passes run every expert layer through moe_few, each to the accuracy of the formula on
+    the rounded weights; the long pass keeps the bits of the default."""
+    from autodiffusion_amd import str_backbone
+    torch.manual_seed(0)
+    kw = dict(hidden_size=128, intermediate_size=256, num_hidden_layers=2, num_attention_heads=8, num_key_value_heads=4, vocab_size=8, precision="bf16")
+    a, b = str_backbone.MixtralModel(**kw).to(dev), str_backbone.MixtralModel(few_token_experts=True, **kw).to(dev)
+    with torch.no_grad():
+        for n, p in a.named_parameters():
+            if p.dim() == 2:
+                p.copy_(torch.randn(p.shape) * p.shape[1] ** -0.5)
+    b.load_state_dict(a.state_dict())
+    calls, plain = [], str_backbone.moe_few
+
+    def recorded(*args):
+        out = plain(*args)
+        calls.append((args, out))
+        return out
+
+    monkeypatch.setattr(str_backbone, "moe_few", recorded)
+    emb = torch.randn(4, 40, 128, device=dev)
+    ca, cb = a.new_cache(), b.new_cache()
+    assert torch.equal(a.extend(emb[:, :37], ca), b.extend(emb[:, :37], cb)) and not calls
+    for i in range(37, 40):
+        a.extend(emb[:, i:i + 1], ca)
+        b.extend(emb[:, i:i + 1], cb)
+    assert len(calls) == 2 * 3                          # layers x passes, of the one model
+    for (x, res, router, s13, s2, inter, E, k, precision, _, _), y in calls:
+        assert precision == "bf16" and x.shape == (4, 128)
+        w13, w2 = (t.view(torch.bfloat16).float().reshape(s) for t, s in ((s13, (E, 2 * inter, 128)), (s2, (E, 128, inter))))
+        want, e, _, _ = moe_exact(x, res, router, w13, w2, k, 2.0 ** -24)
+        within(y, want, e, "fp32", "y")
