@@ -588,13 +588,12 @@ FewPlan few_plan(int T, int d, int inter, int E, int top_k, int act_type, int pr
     FewPlan p;
     const int n = T * top_k, piece = precision == P_F32 ? 32 : 64;
     p.active = n < E ? n : E;                                             // experts that can have been chosen
-    // Both products: two workgroups a CU at most where that leaves none idle -- a workgroup more is a second round for all.
-    // `up`: by the number of waves that share a row group ...
+    // `up`: within UP_BLOCKS by the number of waves that share a row group ...
     const int groups = (inter + 16 * up_nt(T) - 1) / (16 * up_nt(T));
     p.wk = WAVES;
     while (p.wk > 1 && (groups + WAVES / p.wk - 1) / (WAVES / p.wk) * p.active > UP_BLOCKS) p.wk /= 2;
     p.up_blocks = (groups + WAVES / p.wk - 1) / (WAVES / p.wk);
-    // ... `down`: by the number of parts of the hidden axis, each with a piece for every wave
+    // ... `down`: DOWN_BLOCKS and DOWN_KB by the number of parts of the hidden axis, each with a piece for every wave
     p.down_blocks = (d + 16 * down_nt(T) - 1) / (16 * down_nt(T));
     const int64_t bytes = (int64_t)p.active * d * inter * (precision == P_F32 ? 4 : 2) / DOWN_KB >> 10;
     const int want = (int)((bytes > DOWN_BLOCKS ? bytes : DOWN_BLOCKS) / (p.down_blocks * p.active)), most = inter / (piece * WAVES);

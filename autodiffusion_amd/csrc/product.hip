@@ -19,8 +19,8 @@ __device__ __align__(16) unsigned char zero_chunk[16];            // what copies
 
 // ------------------------------------------------------------------------------------------------------------- activations
 // Phi(-|z|), the smaller tail of the normal distribution, and e = exp(-z^2 / 2): e times a polynomial in t = 1 / (1 + 0.35 |z|), fitted to
-// Phi(-|z|) / (t e) for |z| <= 13 (relative error 3e-8, 3e-7 with the roundings in fp32; 1 - erf would have no digits left in the tail).  The
-// slope shares the exponential: the activation of a 256 x 256 tile is as long as a quarter of its products at k = 1024.
+// Phi(-|z|) / (t e) for |z| <= 13 (relative error 8e-8; in fp32 4e-7 up to |z| = 2, then about 6e-8 z^2, 8e-6 at 13, from the roundings of the exponent;
+// absolute at most 1.5e-7; 1 - erf would have no digits left in the tail).  The slope shares the exponential: the activation of a 256 x 256 tile is as long as a quarter of its products at k = 1024.
 __device__ __forceinline__ float normal_tail(float z, float& e) {
     e = exp2_fast(-0.72134752044448170f * z * z);
     const float t = rcp_fast(1.f + 0.35f * fabsf(z));
@@ -563,8 +563,8 @@ __global__ __launch_bounds__(256) void product_join_kernel(const ProductArgs a) 
 }
 
 // ------------------------------------------------------------------------------------------------------------- few rows
-// M <= 64: the weights are read once and everything else is small, so nothing is staged.  A workgroup owns 16 NT rows of w; its
-// waves take 128-byte pieces of K in turn, load fragments of both operands from global memory into registers (16 rows x 16 bytes a
+// M <= 64: the weights are read once and nothing is staged.  A workgroup owns 16 rows of w (and reads all rows of x: 24 x 6144 x 1536
+// moves 28 MB of x from the L2s beside 19 MB of w); its waves take 128-byte pieces of K in turn, load fragments of both operands from global memory into registers (16 rows x 16 bytes a
 // quarter wave) and add up in LDS at the end.
 template <typename T> __device__ __forceinline__ f32x4_t mfma16(const uint4& a, const uint4& b, f32x4_t c) {
     if constexpr (std::is_same<T, __bf16>::value) {
@@ -586,55 +586,46 @@ __device__ __forceinline__ uint4 row_chunk(const T* row, int64_t k, int64_t K) {
     else return unaligned_chunk(row + k, K - k);
 }
 
-template <typename T, int MT, int NT, int NWAVES, bool ALIGNED>
+template <typename T, int MT, int NWAVES, bool ALIGNED>
 __global__ __launch_bounds__(64 * NWAVES) void product_few_kernel(const ProductArgs a) {
     constexpr int CE = 16 / sizeof(T), UNIT = 8 * CE;
-    __shared__ float sums[NWAVES][MT * NT][64][4];
+    __shared__ float sums[NWAVES][MT][64][4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int n0 = blockIdx.x * 16 * NT, r16 = lane & 15, g = lane >> 4;
-    const T *w[NT], *x[MT];
+    const int n0 = blockIdx.x * 16, r16 = lane & 15, g = lane >> 4;
+    const T *w = static_cast<const T*>(a.B) + (int64_t)min(n0 + r16, a.N - 1) * a.ldb + g * CE, *x[MT];
     bool live[MT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) w[t] = static_cast<const T*>(a.B) + (int64_t)min(n0 + t * 16 + r16, a.N - 1) * a.ldb + g * CE;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         live[t] = t * 16 + r16 < a.M;
         x[t] = static_cast<const T*>(a.A) + (int64_t)(live[t] ? t * 16 + r16 : 0) * a.lda + g * CE;
     }
-    f32x4_t acc[NT][MT];
+    f32x4_t acc[MT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < MT; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     const int64_t K = a.K - g * CE;
-    constexpr int U = MT * NT >= 4 ? 2 : 4;                        // pieces in flight a wave
+    constexpr int U = MT >= 4 ? 2 : 4;                             // pieces in flight a wave
     for (int64_t k = (int64_t)wave * UNIT; k < a.K; k += (int64_t)U * NWAVES * UNIT) {
-        uint4 fw[2 * U][NT], fx[2 * U][MT];
+        uint4 fw[2 * U], fx[2 * U][MT];
 #pragma unroll
         for (int h = 0; h < 2 * U; ++h) {
             const int64_t kh = k + (int64_t)(h >> 1) * NWAVES * UNIT + (h & 1) * 4 * CE;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) fw[h][t] = row_chunk<T, ALIGNED>(w[t], kh, K);
+            fw[h] = row_chunk<T, ALIGNED>(w, kh, K);
 #pragma unroll
             for (int t = 0; t < MT; ++t) fx[h][t] = live[t] ? row_chunk<T, ALIGNED>(x[t], kh, K) : make_uint4(0u, 0u, 0u, 0u);
         }
 #pragma unroll
         for (int h = 0; h < 2 * U; ++h)
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int j = 0; j < MT; ++j) acc[i][j] = mfma16<T>(fw[h][i], fx[h][j], acc[i][j]);
+            for (int j = 0; j < MT; ++j) acc[j] = mfma16<T>(fw[h], fx[h][j], acc[j]);
     }
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4_t*>(sums[wave][i * MT + j][lane]) = acc[i][j];
+    for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4_t*>(sums[wave][j][lane]) = acc[j];
     __syncthreads();
     // result layout of the 16x16 product: column (m) = lane & 15, row (n) = 4 (lane >> 4) + reg
-    for (int i = tid; i < MT * NT * 256; i += 64 * NWAVES) {
-        const int nn = i % (16 * NT), m = i / (16 * NT), n = n0 + nn;
+    for (int i = tid; i < MT * 256; i += 64 * NWAVES) {
+        const int nn = i % 16, m = i / 16, n = n0 + nn;
         if (m >= a.M || n >= a.N) continue;
-        const int t = (nn >> 4) * MT + (m >> 4), l = ((nn & 15) >> 2) * 16 + (m & 15), q = nn & 3;
+        const int t = m >> 4, l = (nn >> 2) * 16 + (m & 15), q = nn & 3;
         float v[1] = {0.f};
 #pragma unroll
         for (int s = 0; s < NWAVES; ++s) v[0] += sums[s][t][l][q];
@@ -644,7 +635,7 @@ __global__ __launch_bounds__(64 * NWAVES) void product_few_kernel(const ProductA
 
 // ------------------------------------------------------------------------------------------------------------- gradient of the epilogue
 // dz = dy act'(z), rounded to the operand type of the products that follow, and per chunk of rows the fp32 column sums of the
-// unrounded dz (joined in chunk order: no atomics).
+// unrounded dz (joined in chunk order: no atomics).  Bound: memory; 8192 x 4096 bf16 with fp32 slopes moves 268 MB in 48 us, with codes 201 MB in 42.
 constexpr int SLOPE_ROWS = 64;
 
 template <typename T, typename S, bool VEC>
@@ -736,7 +727,14 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void colsum_join_kernel(const floa
 struct Plan { int tile; int splits; int64_t k_split; size_t part_bytes; };       // tile: 0 few rows, else its edge
 
 // Few rows: the streaming kernel.  Else the largest tile that still gives most CUs one (256: one workgroup a CU, 200 of 256 CUs; 128 and
-// 64: several a CU hide each other's waits).  Tiles of 64 split the summed axis up to four workgroups a CU as long as each keeps 20
+// 64: several a CU hide each other's waits).  Both sides of the borders (us a call, gelu and residual):
+//   64 rows    bf16 x 1024 x 1024: 8 - 64 rows 9 here, 14 in tiles; x 6144 x 1536: 24 rows 9.9 / 13.3, 32 rows 11 / 13.6, 64 rows 17 / 13.8; fp32
+//              x 4096 x 4096: 16 rows 22 / 26, 32 rows 30 / 27, 64 rows 49 / 29 -- above 32 rows the tiles win where w is large
+//   tiles(128) bf16, K = 1024: 2304^2 (324) 25.5 in 128, 29.8 in 64; 2560^2 (400) 26 / 34; K = 4096: 1280^2 (100) 52 / 43, 1792^2 (196) 53 / 68, 2304^2
+//              63 / 97, 2560^2 67 / 115; fp32: 2304^2 140 / 126, 2560^2 141 / 140, 2816^2 142 / 145 -- right for fp32, late for bf16
+//   tiles(256) bf16, K = 1024: 3328^2 (169) 41 in 256, 44 in 128; 3840^2 (225) 44 / 51; 4352^2 (289: a second round) 81 / 67; fp32: 3328^2 264 / 220,
+//              3584^2 (196) 267 / 280, 3840^2 268 / 282, 4352^2 524 / 360 -- the second round of a few tiles is not seen
+// Tiles of 64 split the summed axis up to four workgroups a CU as long as each keeps 20
 // steps of 128 bytes (8 where the tiles alone leave half of the card idle): 1024 x 1024 x 4096 bf16 26 us in one part, 23 in three; the join
 // costs 5 us, so that 1037 x 1024 x 1024 takes 11 us in one part and 15 in two.
 Plan plan_product(int64_t M, int N, int64_t K, int dt, bool acol, bool bcol) {
@@ -765,17 +763,17 @@ template <typename T, bool ACOL, bool BCOL, int EDGE>
 void launch_tile(const ProductArgs& a, hipStream_t s) {
     const int n_tiles = a.tiles_m * a.tiles_n;
     const dim3 grid((unsigned)((n_tiles + 7) / 8 * 8), (unsigned)a.splits);
-    // 256: 238 us for 8192 x 4096 x 4096 bf16 with steps of 128 bytes in two slots, 250 - 270 with 64 in four, 279 with four waves of 128 x 128;
+    // 256: 238 us for 8192 x 4096 x 4096 bf16 (the products alone) with steps of 128 bytes in two slots, 250 - 270 with 64 in four, 279 with four waves of 128 x 128;
     // 64: 26 us for 1024 x 1024 x 4096 with 64 in four, 34 with 128 in two
     constexpr int WN = EDGE == 256 ? 4 : 2, KB = EDGE == 64 ? 64 : 128, R = EDGE == 64 ? 4 : 2;
     hipLaunchKernelGGL((product_kernel<T, ACOL, BCOL, EDGE, EDGE, 2, WN, KB, R>), grid, dim3(128 * WN), 0, s, a);
 }
 
-template <typename T, int MT, int NT, int NWAVES>
+template <typename T, int MT, int NWAVES>
 void launch_few(const ProductArgs& a, bool aligned, hipStream_t s) {
-    const dim3 grid((unsigned)((a.N + 16 * NT - 1) / (16 * NT)));
-    if (aligned) hipLaunchKernelGGL((product_few_kernel<T, MT, NT, NWAVES, true>), grid, dim3(64 * NWAVES), 0, s, a);
-    else hipLaunchKernelGGL((product_few_kernel<T, MT, NT, NWAVES, false>), grid, dim3(64 * NWAVES), 0, s, a);
+    const dim3 grid((unsigned)((a.N + 15) / 16));
+    if (aligned) hipLaunchKernelGGL((product_few_kernel<T, MT, NWAVES, true>), grid, dim3(64 * NWAVES), 0, s, a);
+    else hipLaunchKernelGGL((product_few_kernel<T, MT, NWAVES, false>), grid, dim3(64 * NWAVES), 0, s, a);
 }
 
 inline bool on(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
@@ -801,9 +799,9 @@ hipError_t product(ProductArgs a, int dt, bool acol, bool bcol, bool packed, voi
     if (p.tile == 0) {
         with_dtype(dt, [&](auto t) {
             typedef decltype(t) T;
-            if (a.M <= 16) launch_few<T, 1, 1, 8>(a, pieces, s);
-            else if (a.M <= 32) launch_few<T, 2, 1, 8>(a, pieces, s);
-            else launch_few<T, 4, 1, 8>(a, pieces, s);
+            if (a.M <= 16) launch_few<T, 1, 8>(a, pieces, s);
+            else if (a.M <= 32) launch_few<T, 2, 8>(a, pieces, s);
+            else launch_few<T, 4, 8>(a, pieces, s);
         });
         return hipGetLastError();
     }
