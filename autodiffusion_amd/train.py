@@ -831,12 +831,14 @@ _Accumulator = torch._C._functions.AccumulateGrad
 
 
 def _leaves_on(ctx, what: str, stream: int, capturing) -> None:
-    """The gradient of a leaf is accumulated on the stream of the pass that first reached it, as long as a graph of that pass lives; a capture that
-    is led to another stream ends the process.  Every recorded pass leaves its stream with the accumulators of its leaves, and a
-    capture that finds another one there is refused (passes that reach a leaf by other operators alone leave nothing)."""
+    """The gradient of a leaf is accumulated on the stream of the pass that first reached it, as long as a graph of that pass lives; the default
+    stream (0) takes part in no capture, and a backward pass that is led to it from one ends the process.  Every recorded pass leaves its stream
+    with the accumulators of its leaves, and a capture that finds the default one there is refused (passes that reach a leaf by other
+    operators alone leave nothing; one on a side stream, as warm-up passes are, joins the capture)."""
     for node, _ in ctx.next_functions:
-        if type(node) is _Accumulator and node.metadata.setdefault("adx_stream", stream) != stream and capturing():
-            raise RuntimeError(f"{what}: captured while a graph of an earlier pass over the same leaves is alive: drop its outputs and losses first")
+        if type(node) is _Accumulator and node.metadata.setdefault("adx_stream", stream) == 0 and stream and capturing():
+            raise RuntimeError(f"{what}: captured while a graph of an earlier pass over the same leaves on the default stream is alive: "
+                               "drop its outputs and losses first")
 
 
 def _leaves_on_current(ctx, what: str, device: int) -> None:

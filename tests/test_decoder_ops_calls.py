@@ -109,7 +109,7 @@ def test_forms_of_the_kept_slope():
 
 
 def test_capture_over_the_leaves_of_a_live_graph_is_refused():
-    """On made-up streams: a pass on one stream, then captures on another while its graph lives and after."""
+    """On made-up streams (0: the default one): a pass, then captures while its graph lives and after."""
     class Scaled(torch.autograd.Function):
         @staticmethod
         def forward(ctx, x, stream, capturing):
@@ -121,8 +121,7 @@ def test_capture_over_the_leaves_of_a_live_graph_is_refused():
             return 2 * dy, None, None
 
     w = torch.randn(3, requires_grad=True)
-    y = Scaled.apply(w, 1, False)
-    Scaled.apply(w, 1, True)                                         # the same stream
+    y = Scaled.apply(w, 0, False)
     z = Scaled.apply(w, 2, False)                                    # eager passes on any stream
     with pytest.raises(RuntimeError, match="earlier pass"):
         Scaled.apply(w, 2, True)
@@ -136,3 +135,7 @@ def test_capture_over_the_leaves_of_a_live_graph_is_refused():
     assert torch.equal(torch.autograd.grad((y + z).sum(), w)[0], torch.full((3,), 6.0))
     with torch.no_grad():
         Scaled.apply(w, 3, True)                                     # nothing is recorded
+    del y, z
+    y = Scaled.apply(w, 4, False)                                    # a warm-up on a side stream whose outputs are still held
+    z = Scaled.apply(w, 5, True)
+    assert torch.equal(torch.autograd.grad(z.sum(), w)[0], torch.full((3,), 2.0))
